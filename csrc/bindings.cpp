@@ -10,6 +10,7 @@
 #include <cstdint>
 
 #include "gemm_api.h"
+#include "kv_budget_api.h"
 #include "sched/abi.h"
 #include "sp_api.h"
 
@@ -696,6 +697,279 @@ void moe_combine_norm(int64_t c, int64_t K, at::Tensor &h, const at::Tensor &w, 
   check_rc(rc_, "moe_combine_norm");
 }
 
+// ---------------------------------------------------------------- KV budget (kv_budget_api.h)
+// Shapes and types are checked before devices, so that a wrong call is refused
+// the same way on a machine without a GPU.
+int kv_element(const at::Tensor &t, const char *name) {
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, name, " must be bfloat16 or float16");
+  return t.scalar_type() == at::kHalf ? kKvFp16 : kKvBf16;
+}
+void check_same(const at::Tensor &t, const at::Tensor &as, const char *name) {
+  TORCH_CHECK(t.scalar_type() == as.scalar_type(), name, " must have the cache's type");
+}
+void check_on(const at::Tensor &t, const at::Tensor &as, const char *name) {
+  check_cuda(t, name);
+  TORCH_CHECK(t.device() == as.device(), name, " must be on the cache's device");
+}
+void check_vec(const at::Tensor &t, at::ScalarType type, int64_t n, const char *name, const char *type_name) {
+  TORCH_CHECK(t.scalar_type() == type, name, " must be ", type_name);
+  // (a number streamed into the message crashes the process here; a string does not)
+  TORCH_CHECK(t.dim() == 1 && t.is_contiguous() && t.size(0) >= n, name, " must be contiguous with at least ",
+              std::to_string(n), " entries");
+}
+// k, v [pages, Hkv, page_size, D], contiguous, D 64 or 128
+void check_cache(const at::Tensor &k, const at::Tensor &v) {
+  kv_element(k, "k_cache");
+  check_same(v, k, "v_cache");
+  TORCH_CHECK(k.dim() == 4 && k.is_contiguous() && v.is_contiguous() && v.sizes() == k.sizes(),
+              "k_cache and v_cache must be contiguous [pages, kv heads, page size, head dim] of one shape");
+  TORCH_CHECK(k.size(3) == 64 || k.size(3) == 128, "head dim must be 64 or 128");
+  TORCH_CHECK(k.size(0) >= 1 && k.size(1) >= 1 && k.size(2) >= 1, "the cache must not be empty");
+  TORCH_CHECK(k.size(0) <= INT32_MAX && k.size(1) <= 65535 && k.size(2) <= (1 << 20), "cache dimensions too large");
+}
+// a tracking tensor beside the cache: [pages, Hkv, page_size], contiguous
+void check_track(const at::Tensor &t, const at::Tensor &k, at::ScalarType type, const char *name, const char *type_name) {
+  TORCH_CHECK(t.scalar_type() == type, name, " must be ", type_name);
+  TORCH_CHECK(t.dim() == 3 && t.is_contiguous() && t.size(0) == k.size(0) && t.size(1) == k.size(1) &&
+                  t.size(2) == k.size(2),
+              name, " must be contiguous [pages, kv heads, page size]");
+}
+void check_table(const at::Tensor &bt, int64_t rows) {
+  TORCH_CHECK(bt.scalar_type() == at::kInt, "block_table must be int32");
+  TORCH_CHECK(bt.dim() == 2 && bt.size(0) >= rows && bt.size(1) >= 1 && bt.stride(1) == 1 && bt.size(1) <= INT32_MAX,
+              "block_table must be [>= requests, pages per request] with contiguous rows");
+}
+void check_aligned(const at::Tensor &t, const char *name) {
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name, " must start on a 16-byte boundary");
+}
+
+void qk_norm_rope_kv_append(const at::Tensor &qkv, const at::Tensor &wq, const at::Tensor &wk, double eps,
+                            const at::Tensor &pos, const at::Tensor &slot, const at::Tensor &cos_sin, at::Tensor &q_out,
+                            at::Tensor &k_cache, at::Tensor &v_cache, int64_t Hq, int64_t Hkv,
+                            const c10::optional<at::Tensor> &scores, const c10::optional<at::Tensor> &positions,
+                            const c10::optional<at::Tensor> &status) {
+  check_cache(k_cache, v_cache);
+  const int64_t D = k_cache.size(3);
+  TORCH_CHECK(Hkv == k_cache.size(1), "n_kv_heads must be the cache's");
+  TORCH_CHECK(Hq >= 1 && Hq <= 65535, "n_q_heads must be positive");
+  check_same(qkv, k_cache, "qkv");
+  TORCH_CHECK(qkv.dim() == 2 && qkv.size(1) == (Hq + 2 * Hkv) * D && (qkv.stride(1) == 1 || qkv.size(0) == 0),
+              "qkv must be [tokens, (q heads + 2 kv heads) * head dim] with contiguous rows");
+  const int64_t T = qkv.size(0);
+  TORCH_CHECK(T <= INT32_MAX && T * (Hq + 2 * Hkv) <= INT32_MAX, "too many tokens in one call");
+  check_same(wq, k_cache, "q_weight");
+  check_same(wk, k_cache, "k_weight");
+  TORCH_CHECK(wq.dim() == 1 && wk.dim() == 1 && wq.size(0) == D && wk.size(0) == D && wq.is_contiguous() &&
+                  wk.is_contiguous(),
+              "q_weight and k_weight must be contiguous [head dim]");
+  check_vec(pos, at::kInt, T, "pos", "int32");
+  check_vec(slot, at::kInt, T, "slot", "int32");
+  TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.dim() == 3 && cos_sin.is_contiguous() &&
+                  cos_sin.size(2) == 2 && cos_sin.size(0) >= 1 && cos_sin.size(0) <= INT32_MAX,
+              "cos_sin must be contiguous float32 [positions, rotated dims / 2, 2]");
+  const int64_t rot = 2 * cos_sin.size(1);
+  TORCH_CHECK(rot >= 16 && rot <= D && rot % 16 == 0, "the rotated dims must be a multiple of 16, at most the head dim");
+  check_same(q_out, k_cache, "q_out");
+  TORCH_CHECK(q_out.dim() == 3 && q_out.size(0) >= T && q_out.size(1) == Hq && q_out.size(2) == D &&
+                  q_out.stride(2) == 1 && (q_out.stride(1) == D || Hq == 1),
+              "q_out must be [>= tokens, q heads, head dim] with contiguous heads");
+  if (scores.has_value()) check_track(*scores, k_cache, at::kFloat, "scores", "float32");
+  if (positions.has_value()) check_track(*positions, k_cache, at::kInt, "positions", "int32");
+  // a slot is an int32: the whole cache must be addressable by one
+  TORCH_CHECK(T <= 1 || (qkv.stride(0) % 8 == 0 && q_out.stride(0) % 8 == 0 && q_out.stride(0) >= Hq * D),
+              "rows of qkv and q_out must not overlap and must start on 16-byte boundaries");
+  const std::pair<const at::Tensor *, const char *> on[] = {{&qkv, "qkv"}, {&wq, "q_weight"}, {&wk, "k_weight"},
+      {&pos, "pos"}, {&slot, "slot"}, {&cos_sin, "cos_sin"}, {&q_out, "q_out"}, {&v_cache, "v_cache"}};
+  check_cuda(k_cache, "k_cache");
+  for (const auto &t : on) check_on(*t.first, k_cache, t.second);
+  if (scores.has_value()) check_on(*scores, k_cache, "scores");
+  if (positions.has_value()) check_on(*positions, k_cache, "positions");
+  if (T == 0) return;
+  for (const auto &t : on)
+    if (t.first != &pos && t.first != &slot) check_aligned(*t.first, t.second);
+  check_aligned(k_cache, "k_cache");
+  QkNormArgs a{};
+  a.qkv = qkv.data_ptr();
+  a.ld_qkv = T > 1 ? qkv.stride(0) : 0;
+  a.wq = wq.data_ptr();
+  a.wk = wk.data_ptr();
+  a.eps = (float)eps;
+  a.pos = pos.data_ptr<int32_t>();
+  a.slot = slot.data_ptr<int32_t>();
+  a.cos_sin = cos_sin.data_ptr<float>();
+  a.max_pos = cos_sin.size(0);
+  a.rot = rot;
+  a.q_out = q_out.data_ptr();
+  a.ld_q = T > 1 ? q_out.stride(0) : 0;
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v_cache.data_ptr();
+  a.scores = ptr_or_null<float>(scores);
+  a.positions = ptr_or_null<int32_t>(positions);
+  a.T = T;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.D = D;
+  a.page_size = k_cache.size(2);
+  a.num_pages = k_cache.size(0);
+  a.element = kv_element(k_cache, "k_cache");
+  a.status = ptr_or_null<int>(status);
+  int rc_ = 0;
+  {  // the guard is gone before check_rc may throw
+    c10::cuda::CUDAGuard g(k_cache.device());
+    rc_ = sched_qk_norm_rope_kv_append(&a, cur_stream());
+  }
+  check_rc(rc_, "qk_norm_rope_kv_append");
+}
+
+// q, out [R, Q, Hq, D]; lse [R, Q, Hq]
+void attn_decode_scored(const at::Tensor &q, at::Tensor &out, const at::Tensor &k_cache, const at::Tensor &v_cache,
+                        const at::Tensor &block_table, const at::Tensor &kv_lens, double sm_scale, at::Tensor &scores,
+                        const c10::optional<at::Tensor> &lse, int64_t max_len, const c10::optional<at::Tensor> &status) {
+  check_cache(k_cache, v_cache);
+  const int64_t D = k_cache.size(3), Hkv = k_cache.size(1), ps = k_cache.size(2);
+  TORCH_CHECK(ps % 16 == 0, "the page size must be a multiple of 16");
+  check_same(q, k_cache, "q");
+  check_same(out, k_cache, "out");
+  TORCH_CHECK(q.dim() == 4 && q.size(3) == D && q.size(2) >= 1 && q.size(2) % Hkv == 0,
+              "q must be [requests, queries, q heads, head dim] with q heads a multiple of the cache's heads");
+  TORCH_CHECK(out.sizes() == q.sizes(), "out must have q's shape");
+  const int64_t R = q.size(0), Q = q.size(1), Hq = q.size(2);
+  for (const at::Tensor *t : {&q, (const at::Tensor *)&out})
+    TORCH_CHECK(t->numel() == 0 || (t->stride(3) == 1 && (t->stride(2) == D || Hq == 1) &&
+                                    (Q == 1 || t->stride(1) % 8 == 0) && (R == 1 || t->stride(0) % 8 == 0)),
+                "q and out need contiguous heads and rows on 16-byte boundaries");
+  TORCH_CHECK(out.numel() == 0 || ((Q == 1 || out.stride(1) >= Hq * D) && (R == 1 || out.stride(0) >= Hq * D)),
+              "rows of out must not overlap");
+  TORCH_CHECK(R <= 65535 && Q * (Hq / Hkv) <= 8192, "at most 65535 requests and 8192 query rows per KV head");
+  check_table(block_table, R);
+  check_vec(kv_lens, at::kInt, R, "kv_lens", "int32");
+  check_track(scores, k_cache, at::kFloat, "scores", "float32");
+  if (lse.has_value()) {
+    TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->dim() == 3 && lse->size(0) == R &&
+                    lse->size(1) == Q && lse->size(2) == Hq,
+                "lse must be contiguous float32 [requests, queries, q heads]");
+  }
+  TORCH_CHECK(max_len >= 0, "max_len must not be negative");
+  int64_t cap = block_table.size(1) * ps;
+  if (max_len > 0 && max_len < cap) cap = max_len;
+  TORCH_CHECK(cap <= INT32_MAX - 1024, "contexts of 2^31 tokens or more");
+  check_cuda(k_cache, "k_cache");
+  const std::pair<const at::Tensor *, const char *> on[] = {{&q, "q"}, {&out, "out"}, {&v_cache, "v_cache"},
+      {&block_table, "block_table"}, {&kv_lens, "kv_lens"}, {&scores, "scores"}};
+  for (const auto &t : on) check_on(*t.first, k_cache, t.second);
+  if (lse.has_value()) check_on(*lse, k_cache, "lse");
+  if (R == 0 || Q == 0) return;
+  check_aligned(q, "q");
+  check_aligned(k_cache, "k_cache");
+  check_aligned(v_cache, "v_cache");
+  check_aligned(scores, "scores");
+  ScoredArgs a{};
+  a.q = q.data_ptr();
+  a.q_req = R > 1 ? q.stride(0) : 0;
+  a.q_query = Q > 1 ? q.stride(1) : 0;
+  a.out = out.data_ptr();
+  a.out_req = R > 1 ? out.stride(0) : 0;
+  a.out_query = Q > 1 ? out.stride(1) : 0;
+  a.lse = ptr_or_null<float>(lse);
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v_cache.data_ptr();
+  a.scores = scores.data_ptr<float>();
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.bt_stride = block_table.stride(0);
+  a.bt_pages = block_table.size(1);
+  a.kv_lens = kv_lens.data_ptr<int32_t>();
+  a.R = R;
+  a.Q = Q;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.D = D;
+  a.page_size = ps;
+  a.num_pages = k_cache.size(0);
+  a.max_len = cap;
+  a.element = kv_element(k_cache, "k_cache");
+  a.num_sms = num_sms(k_cache);
+  a.sm_scale = (float)sm_scale;
+  a.status = ptr_or_null<int>(status);
+  int rc_ = 0;
+  {  // the guard is gone before check_rc may throw
+    c10::cuda::CUDAGuard g(k_cache.device());
+    // scratch of this call alone, from the allocator's pool of the current stream (or of the graph being captured)
+    const long long floats = sched_attn_scored_ws_floats(a.R, a.Q, a.Hq, a.Hkv, a.D, a.max_len, a.num_sms);
+    at::Tensor ws = at::empty({floats}, scores.options());
+    a.ws = ws.data_ptr<float>();
+    a.ws_floats = floats;
+    rc_ = sched_attn_scored(&a, cur_stream());
+  }
+  check_rc(rc_, "attn_decode_scored");
+}
+
+void kv_evict(at::Tensor &k_cache, at::Tensor &v_cache, at::Tensor &scores, at::Tensor &positions,
+              const at::Tensor &block_table, const at::Tensor &kv_lens, const at::Tensor &last_pos, int64_t budget,
+              int64_t recent, int64_t sink, at::Tensor &new_lens, int64_t max_len,
+              const c10::optional<at::Tensor> &status) {
+  check_cache(k_cache, v_cache);
+  const int64_t ps = k_cache.size(2);
+  check_track(scores, k_cache, at::kFloat, "scores", "float32");
+  check_track(positions, k_cache, at::kInt, "positions", "int32");
+  TORCH_CHECK(kv_lens.dim() == 1, "kv_lens must be [requests]");
+  const int64_t R = kv_lens.size(0);
+  check_vec(kv_lens, at::kInt, R, "kv_lens", "int32");
+  check_vec(last_pos, at::kInt, R, "last_pos", "int32");
+  check_vec(new_lens, at::kInt, R, "new_lens", "int32");
+  check_table(block_table, R);
+  TORCH_CHECK(R <= 65535, "at most 65535 requests");
+  TORCH_CHECK(budget >= 1 && budget <= INT32_MAX, "budget must be at least 1");
+  TORCH_CHECK(recent >= 0 && sink >= 0 && recent <= budget && sink <= budget && recent + sink <= budget,
+              "recent and sink must not be negative, and together at most the budget");
+  TORCH_CHECK(max_len >= 0, "max_len must not be negative");
+  int64_t cap = block_table.size(1) * ps;
+  if (max_len > 0 && max_len < cap) cap = max_len;
+  TORCH_CHECK(cap <= INT32_MAX - 1024, "contexts of 2^31 tokens or more");
+  check_cuda(k_cache, "k_cache");
+  const std::pair<const at::Tensor *, const char *> on[] = {{&v_cache, "v_cache"}, {&scores, "scores"},
+      {&positions, "positions"}, {&block_table, "block_table"}, {&kv_lens, "kv_lens"}, {&last_pos, "last_pos"},
+      {&new_lens, "new_lens"}};
+  for (const auto &t : on) check_on(*t.first, k_cache, t.second);
+  if (R == 0) return;
+  const int32_t *nl = new_lens.data_ptr<int32_t>(), *kl = kv_lens.data_ptr<int32_t>(), *lp = last_pos.data_ptr<int32_t>();
+  TORCH_CHECK((nl + R <= kl || kl + R <= nl) && (nl + R <= lp || lp + R <= nl),
+              "new_lens must not overlap kv_lens or last_pos: every head reads the old ones");
+  check_aligned(k_cache, "k_cache");
+  check_aligned(v_cache, "v_cache");
+  KvEvictArgs a{};
+  a.k_cache = k_cache.data_ptr();
+  a.v_cache = v_cache.data_ptr();
+  a.scores = scores.data_ptr<float>();
+  a.positions = positions.data_ptr<int32_t>();
+  a.block_table = block_table.data_ptr<int32_t>();
+  a.bt_stride = block_table.stride(0);
+  a.bt_pages = block_table.size(1);
+  a.kv_lens = kv_lens.data_ptr<int32_t>();
+  a.last_pos = last_pos.data_ptr<int32_t>();
+  a.new_lens = new_lens.data_ptr<int32_t>();
+  a.R = R;
+  a.Hkv = k_cache.size(1);
+  a.D = k_cache.size(3);
+  a.page_size = ps;
+  a.num_pages = k_cache.size(0);
+  a.max_len = cap;
+  a.budget = budget;
+  a.recent = recent;
+  a.sink = sink;
+  a.num_sms = num_sms(k_cache);
+  a.status = ptr_or_null<int>(status);
+  int rc_ = 0;
+  {  // the guard is gone before check_rc may throw
+    c10::cuda::CUDAGuard g(k_cache.device());
+    const long long ints = sched_kv_evict_ws_ints(a.R, a.Hkv, a.max_len, a.budget);
+    at::Tensor ws = at::empty({ints}, kv_lens.options());
+    a.ws = ints > 0 ? ws.data_ptr<int32_t>() : nullptr;
+    a.ws_ints = ints;
+    rc_ = sched_kv_evict(&a, cur_stream());
+  }
+  check_rc(rc_, "kv_evict");
+}
+
 void probe_stream(const at::Tensor &src, int64_t policy, at::Tensor &sink, int64_t grid) {
   TORCH_CHECK(src.is_cuda() && src.is_contiguous(), "src on the device");
   int rc_ = 0;
@@ -871,6 +1145,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_ws_floats", &gemm_ws_floats);
   m.def("attn_decode", &attn_decode);
   m.def("attn_merge", &attn_merge);
+  m.def("qk_norm_rope_kv_append", &qk_norm_rope_kv_append);
+  m.def("attn_decode_scored", &attn_decode_scored);
+  m.def("kv_evict", &kv_evict);
   m.def("attn_prefill", &attn_prefill);
   m.def("attn_prefill_tile_rows", &sched_attn_prefill_tile_rows);
   m.def("attn_decode_occupancy", &attn_decode_occupancy);

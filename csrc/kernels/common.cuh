@@ -30,6 +30,11 @@ enum IndexSite : int {
   kSiteTokenId = 4,       // embedding: token id
   kSiteDecodePage = 5,    // decode attention: block-table page id
   kSitePrefillPage = 6,   // prefill attention: block-table page id
+  kSiteNormPos = 7,       // per-head norm + rotation: position of a token
+  kSiteScoredPage = 8,    // scored decode attention: block-table page id
+  kSiteScoredLen = 9,     // scored decode attention: KV length
+  kSiteEvictPage = 10,    // eviction: block-table page id
+  kSiteEvictLen = 11,     // eviction: KV length
 };
 
 // A status buffer holds 4 int32 words: [0] the code, and for

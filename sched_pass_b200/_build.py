@@ -39,6 +39,7 @@ KERNEL_SOURCES = [
     "kernels/attention_decode.cu",
     "kernels/attention_prefill.cu",
     "kernels/elementwise.cu",
+    "kernels/kv_budget.cu",
     "kernels/moe.cu",
     "kernels/kv_tier.cu",
     "kernels/microbench.cu",

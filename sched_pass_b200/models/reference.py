@@ -1,4 +1,4 @@
-"""Plain-PyTorch fp32 statements of every kernel, used as test oracles.
+"""Plain-PyTorch statements of every kernel (fp32; 64 bits where said), used as test oracles.
 
 These are definitions, not a fallback: nothing in the serving path calls
 them. Each mirrors one native kernel's contract exactly (layouts included).
@@ -79,6 +79,83 @@ def decode_attention_paged(q, k_cache, v_cache, block_table, seq_lens, sm_scale,
         tau = int(taus[b]) if taus is not None else 0
         outs.append(attention(q[b:b + 1], k, v, sm_scale, tau=tau)[0])
     return torch.stack(outs)
+
+
+def qk_norm_rope(x, weight, eps, pos, cos_sin):
+    """RMSNorm of each head, then rotation of the first 2 * cos_sin.shape[1]
+    values; x [T, H, D]; in 64 bits."""
+    x = x.double()
+    y = x / torch.sqrt(x.pow(2).mean(-1, keepdim=True) + eps) * weight.double()
+    half = cos_sin.shape[1]
+    cs = cos_sin.double()[pos.long()][:, None]
+    a, b = y[..., :half], y[..., half:2 * half]
+    return torch.cat([a * cs[..., 0] - b * cs[..., 1], b * cs[..., 0] + a * cs[..., 1], y[..., 2 * half:]], -1)
+
+
+def attention_scored(q, k_cache, v_cache, block_table, kv_lens, sm_scale):
+    """q [R, Q, Hq, D], the last Q tokens of each request; in 64 bits. Returns
+    (out, lse [R, Q, Hq], weights: per request [Hkv, its length]), where a
+    token in a page outside the cache has weight 0."""
+    R, Q, Hq, D = q.shape
+    P, Hkv, ps, _ = k_cache.shape
+    out = torch.zeros(R, Q, Hq, D, dtype=torch.float64, device=q.device)
+    lse = torch.full((R, Q, Hq), -math.inf, dtype=torch.float64, device=q.device)
+    weights = []
+    for r in range(R):
+        n = int(kv_lens[r])
+        w = torch.zeros(Hkv, n, dtype=torch.float64, device=q.device)
+        weights.append(w)
+        if n == 0:
+            continue
+        page = block_table[r, : (n + ps - 1) // ps].long()
+        there = ((page >= 0) & (page < P)).repeat_interleave(ps)[:n]
+        page = page.clamp(0, P - 1)
+        k = k_cache[page].transpose(0, 1).reshape(Hkv, -1, D)[:, :n].double()
+        v = v_cache[page].transpose(0, 1).reshape(Hkv, -1, D)[:, :n].double()
+        for i in range(Q):
+            see = there & (torch.arange(n, device=q.device) < n - (Q - 1 - i))
+            if not bool(see.any()):
+                continue
+            s = torch.einsum("hgd,hnd->hgn", q[r, i].double().view(Hkv, -1, D), k[:, see]) * sm_scale
+            z = torch.logsumexp(s, -1)
+            p = torch.exp(s - z[..., None])
+            out[r, i] = torch.einsum("hgn,hnd->hgd", p, v[:, see]).reshape(Hq, D)
+            lse[r, i] = z.reshape(-1)
+            w[:, see] += p.sum(1)
+    return out, lse, weights
+
+
+def kv_evict(k_cache, v_cache, scores, positions, block_table, kv_lens, last_pos, budget, recent, sink=0):
+    """The eviction's outcome as new tensors: (k, v, scores, positions,
+    lengths). Tokens in pages outside the cache go first and are not moved."""
+    P, Hkv, ps, D = k_cache.shape
+    new = [t.clone().cpu() for t in (k_cache, v_cache, scores, positions)]
+    flat = [new[0].view(-1, D), new[1].view(-1, D), new[2].view(-1), new[3].view(-1)]
+    score, pos = flat[2].double().tolist(), flat[3].tolist()
+    table, lens, last = block_table.cpu().tolist(), kv_lens.cpu().tolist(), last_pos.cpu().tolist()
+    for r, n in enumerate(lens):
+        if n <= budget:
+            continue
+        for h in range(Hkv):
+            row = [-1 if not 0 <= table[r][j // ps] < P else (table[r][j // ps] * Hkv + h) * ps + j % ps for j in range(n)]
+
+            def rank(j):
+                if row[j] < 0:
+                    return (3, 0.0, j)
+                x = score[row[j]]
+                if pos[row[j]] > last[r] - recent or pos[row[j]] < sink:
+                    return (0, 0.0, j)
+                return (1, -x, j) if x == x else (1, math.inf, j)
+
+            kept = set(sorted(range(n), key=rank)[:budget])
+            movers = [j for j in range(budget, n) if j in kept]
+            holes = [j for j in range(budget) if j not in kept]
+            pairs = [(row[a], row[b]) for a, b in zip(movers, holes) if row[a] >= 0 and row[b] >= 0]
+            if pairs:
+                src, dst = (torch.tensor(x) for x in zip(*pairs))
+                for t in flat:
+                    t[dst] = t[src]
+    return tuple(t.to(k_cache.device) for t in new) + (torch.clamp(kv_lens, max=budget),)
 
 
 def llama_forward_tokens(cfg, weights, token_ids, cos_sin):

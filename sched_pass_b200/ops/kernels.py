@@ -31,7 +31,9 @@ STATUS_NAMES = {0: "ok", 1: "tma-timeout", 2: "mma-timeout", 3: "epilogue-timeou
                 4: "peer-timeout", 5: "clc-timeout", 6: "bad-argument", 7: "bad-index"}
 INDEX_SITES = {1: "kv page copy: source page", 2: "kv page copy: destination page", 3: "KV append: cache slot",
                4: "embedding: token id", 5: "decode attention: block-table page",
-               6: "prefill attention: block-table page"}
+               6: "prefill attention: block-table page", 7: "per-head norm + rotation: position",
+               8: "scored decode attention: block-table page", 9: "scored decode attention: KV length",
+               10: "eviction: block-table page", 11: "eviction: KV length"}
 # the wait that gave up, for timeouts that record it
 WAIT_SITES = {101: "decode producer: task slot free", 102: "decode MMA: task published",
               103: "decode MMA: query rows staged", 104: "decode MMA: task's O buffer free",
@@ -213,6 +215,88 @@ def attention_decode(q, out, k_cache, v_cache, block_table, items, num_items, sm
                       int(grid), int(pf_blocks), float(dT), float(dR), float(H), sk, sv, int(split),
                       status_buffer(q.device), int(pf_ptr), int(pf_bytes))
     return out
+
+
+def _status_of(t: torch.Tensor) -> torch.Tensor | None:
+    # a CPU tensor is refused by the binding, with its name
+    return status_buffer(t.device) if t.is_cuda else None
+
+
+def qk_norm_rope_kv_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float,
+                           pos: torch.Tensor, slot: torch.Tensor, cos_sin: torch.Tensor, q_out: torch.Tensor,
+                           k_cache: torch.Tensor, v_cache: torch.Tensor, n_q_heads: int, n_kv_heads: int, *,
+                           scores: torch.Tensor | None = None, positions: torch.Tensor | None = None) -> torch.Tensor:
+    """``rope_kv_append`` with an RMSNorm of every query and key head before
+    the rotation, in the same pass: y = x * rsqrt(mean(x^2) + eps) * weight
+    over the head's values, then the first 2 * cos_sin.shape[1] of them turn in
+    pairs (d, d + half); value heads are copied. fp32 throughout, rounded once.
+
+    qkv [T, (Hq + 2 Hkv) * D] (rows may be strided), weights [D], q_out
+    [>= T, Hq, D], caches [pages, Hkv, page_size, D], all bf16 or all fp16,
+    D 64 or 128. ``slot`` < 0 writes no cache entry. Two tokens of one call
+    must not name the same slot. ``scores`` float32 and ``positions`` int32
+    [pages, Hkv, page_size] start the tracking of the new slots for
+    ``attention_decode_scored`` and ``kv_evict``: weight 0, the token's
+    position. A position outside the table zeroes the token's q row, a bad
+    position or slot skips its cache writes; both are reported (``check_status``)."""
+    ext().qk_norm_rope_kv_append(qkv, q_weight, k_weight, float(eps), pos, slot, cos_sin, q_out, k_cache, v_cache,
+                                 int(n_q_heads), int(n_kv_heads), scores, positions, _status_of(k_cache))
+    return q_out
+
+
+def attention_decode_scored(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            block_table: torch.Tensor, kv_lens: torch.Tensor, sm_scale: float, scores: torch.Tensor, *,
+                            lse: torch.Tensor | None = None, max_len: int = 0) -> torch.Tensor:
+    """Attention of the newest tokens over the paged cache that also adds to
+    ``scores`` (float32 [pages, Hkv, page_size]), for every cached token and KV
+    head, the weight that this call's queries gave it, summed over the queries
+    and the query heads of that KV head: what ``kv_evict`` selects by.
+
+    q and out [R, Hq, D] (one new token per request) or [R, Q, Hq, D]: the last
+    Q tokens of each request, each seeing itself and what is before it (query i
+    sees the first kv_lens[r] - (Q - 1 - i) tokens), e.g. the end of a prompt,
+    whose weights start its tokens' scores. A row that sees nothing gives zeros
+    and lse = -inf. ``lse`` float32 of q's shape without D: natural log of the
+    softmax's sum. ``max_len``: a bound of the kv_lens that the host knows
+    (0: the block table's width); it sizes the scratch, and a longer length is
+    reported and cut. bf16 or fp16, D 64 or 128, page size a multiple of 16,
+    any Hq / Hkv.
+
+    The pages of one call's requests should be distinct: in a page that two
+    requests share, both add their weights, in no fixed order. Pages outside
+    the cache are reported and left out."""
+    q4, o4 = (q.unsqueeze(1), out.unsqueeze(1)) if q.dim() == 3 and out.dim() == 3 else (q, out)
+    l3 = lse.unsqueeze(1) if lse is not None and q.dim() == 3 and lse.dim() == 2 else lse
+    ext().attn_decode_scored(q4, o4, k_cache, v_cache, block_table, kv_lens, float(sm_scale), scores, l3, int(max_len),
+                             _status_of(k_cache))
+    return out
+
+
+def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor, positions: torch.Tensor,
+             block_table: torch.Tensor, kv_lens: torch.Tensor, last_pos: torch.Tensor, budget: int, recent: int, *,
+             sink: int = 0, max_len: int = 0, new_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """Cut every request of more than ``budget`` cached tokens back to
+    ``budget``, in place, for each KV head by itself. Kept are the tokens of
+    the last ``recent`` positions (position > last_pos[r] - recent), those of
+    position < ``sink``, and of the rest the ones with the largest ``scores``,
+    the lowest slot first among equals (NaN counts as -inf).
+
+    The kept tokens of the slots from ``budget`` on move into the slots below
+    it whose tokens go, the i-th into the i-th; every other entry of the caches
+    and of ``scores`` / ``positions`` [pages, Hkv, page_size] stays as it was.
+    The order of the slots is then no longer that of the positions (attention
+    does not need it: keys carry their rotation; ``positions`` keeps track).
+    Returns the new lengths, int32 [R] = min(kv_lens, budget): further tokens
+    are appended from there, and the pages behind are free. The cache is not
+    read where a request fits its budget. ``max_len`` as in
+    ``attention_decode_scored``. Pages must not be shared by requests (nor with
+    a prefix cache). Pages outside the cache are reported; their tokens go
+    first and are not moved."""
+    if new_lens is None:
+        new_lens = torch.empty(kv_lens.shape[0] if kv_lens.dim() else 0, dtype=torch.int32, device=kv_lens.device)
+    ext().kv_evict(k_cache, v_cache, scores, positions, block_table, kv_lens, last_pos, int(budget), int(recent),
+                   int(sink), new_lens, int(max_len), _status_of(k_cache))
+    return new_lens
 
 
 def attention_merge(part_o, part_lse, merge_req, merge_begin, rows, out):
