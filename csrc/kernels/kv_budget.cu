@@ -167,30 +167,41 @@ __global__ void __launch_bounds__(256) qk_norm_kernel(const QkNormArgs a) {
 // the s_ij are kept (fp32, in units of log 2): 4 Q G bytes a token and KV head
 // beside the 4 D bytes of K and V that the pass has to read.
 //
-// The tokens of a request are cut into chunks, a CTA each; a second kernel
-// joins the chunks' partial results and adds the weights.
+// Work is cut evenly over warps, not over requests: the 16-token tiles of all
+// (request, KV head, row block) tasks form one list, and every warp takes an
+// equal run of it, whatever the lengths. A run's part of a task leaves a
+// partial result (max, sum, output) in the workspace; a second kernel joins
+// them and adds the weights. Runs and tasks advance together through the
+// list, so (warp + task) numbers the partial results without gaps to look up.
 constexpr int kWarps = 4;      // per CTA of the split kernel
 constexpr int kTile = 16;      // tokens per warp step: divides the page size
+constexpr int kResident = 3;   // CTAs of the split kernel per SM
+constexpr int kMinRun = 2;     // tiles per warp at least: bounds the partial results
 
 struct ScoredPlan {
-  int rows, lp, chunk, nch;  // query rows per KV head, padded length, tokens per chunk, chunks
+  int rows, lp;         // query rows per KV head, padded length
+  int block, blocks;    // rows per task (8 or 16), tasks per (request, KV head)
+  int grid, join;       // CTAs of the split kernel, tokens per CTA of the join
   long long s_off, o_off, ml_off, total;
 };
 
-// Chunks of up to 512 tokens; shorter while the grid would leave SMs idle.
 inline ScoredPlan scored_plan(int R, int Q, int Hq, int Hkv, int D, int max_len, int num_sms) {
   ScoredPlan p;
   p.rows = Q * (Hq / Hkv);
   p.lp = (max_len + kTile - 1) / kTile * kTile;
-  const long long blocks = (long long)R * Hkv * ((p.rows + 15) / 16);
-  p.chunk = 512;
-  while (p.chunk > kWarps * kTile && blocks * ((max_len + p.chunk - 1) / p.chunk) < 4ll * num_sms) p.chunk /= 2;
-  p.nch = (max_len + p.chunk - 1) / p.chunk;
-  const long long heads = (long long)R * Hkv;
+  p.block = p.rows <= 8 ? 8 : 16;
+  p.blocks = (p.rows + p.block - 1) / p.block;
+  const long long heads = (long long)R * Hkv, tasks = heads * p.blocks;
+  const long long most = (tasks * (p.lp / kTile) + kMinRun * kWarps - 1) / (kMinRun * kWarps);
+  const long long fill = (long long)num_sms * kResident;
+  p.grid = (int)(most < fill ? most : fill);
+  p.join = 2048;
+  while (p.join > 256 && heads * ((max_len + p.join - 1) / p.join) < num_sms) p.join /= 2;
   p.s_off = 0;
   p.o_off = heads * p.rows * p.lp;
-  p.ml_off = p.o_off + heads * p.nch * p.rows * D;
-  p.total = p.ml_off + heads * p.nch * p.rows * 2;
+  const long long parts = (long long)p.grid * kWarps + tasks;
+  p.ml_off = p.o_off + parts * p.block * D;
+  p.total = p.ml_off + parts * p.block * 2;
   return p;
 }
 
@@ -229,104 +240,112 @@ __device__ __forceinline__ int checked_len(int n, int cap, int *status, int site
   }
   return n < 0 ? 0 : n;
 }
+__device__ __forceinline__ int table_cap(int max_len, int pages, int page_size) {
+  return (int)min((long long)max_len, (long long)pages * page_size);
+}
 
 // exp2(m - ref) with m = -inf or an empty row's ref = -inf giving 0
 __device__ __forceinline__ float scale_to(float m, float ref) { return ref == -INFINITY ? 0.f : ex2_approx(m - ref); }
 
-// o += P V for one tile: this lane's V values of tokens 2c, 2c+1, 8+2c, 9+2c
-// (vt[i][.]), D in 64-value halves i. ROWS 8: rows 8-15 of the product are
-// not used. The column n of product (i, e) is value 64 i + 8 n + e of the
-// head, so that a lane's 16 bytes of V feed eight products.
-template <typename T, int D, int ROWS>
-__device__ __forceinline__ void add_pv(float (&o)[D / 8][ROWS / 4], const uint4 (&vt)[D / 64][4], uint32_t a0, uint32_t a1,
-                                       uint32_t a2, uint32_t a3) {
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const uint32_t t0[4] = {vt[i][0].x, vt[i][0].y, vt[i][0].z, vt[i][0].w};
-    const uint32_t t1[4] = {vt[i][1].x, vt[i][1].y, vt[i][1].z, vt[i][1].w};
-    const uint32_t t2[4] = {vt[i][2].x, vt[i][2].y, vt[i][2].z, vt[i][2].w};
-    const uint32_t t3[4] = {vt[i][3].x, vt[i][3].y, vt[i][3].z, vt[i][3].w};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
-      const uint32_t b0 = __byte_perm(t0[e / 2], t1[e / 2], sel), b1 = __byte_perm(t2[e / 2], t3[e / 2], sel);
-      float(&acc)[ROWS / 4] = o[i * 8 + e];
-      if constexpr (ROWS == 16) {
-        mma16816<T>(acc[0], acc[1], acc[2], acc[3], a0, a1, a2, a3, b0, b1);
-      } else {
-        float z0 = 0.f, z1 = 0.f;
-        mma16816<T>(acc[0], acc[1], z0, z1, a0, 0u, a2, 0u, b0, b1);
-      }
-    }
-  }
+// Tiles per warp of the split kernel, for the list's total.
+__device__ __forceinline__ uint32_t run_length(uint32_t total, uint32_t warps) {
+  const uint32_t per = (total + warps - 1) / warps;
+  return per < kMinRun ? kMinRun : per;
 }
 
 __device__ __forceinline__ uint4 keep_if(bool k, const uint4 &v) { return k ? v : make_uint4(0, 0, 0, 0); }
 
-// One CTA: a chunk of one request's tokens for one KV head and ROWS of its
-// query rows. Each warp takes every fourth 16-token tile and keeps its own
-// running maximum, sum and output; K and V go from global memory straight
-// into the registers of the m16n8k16 operands (the next tile's loads are in
-// flight while this one is used), so there is no shared-memory staging.
+// One warp: a run of tiles. K and V go from global memory straight into the
+// registers of the m16n8k16 operands (K of the next tile is requested once
+// this one's logits are done, V once its product is), so a warp always has
+// loads in flight and there is no shared-memory staging; Q waits in shared
+// memory in operand order. Query rows are the M side (8 of its 16 rows where
+// a KV head has at most 8 query rows), tokens the N side of the logits and
+// the K side of the output.
+//
+// Operand layout, for lane 4 r + c: the 16 bytes of K at value 32 kk + 8 c of
+// tokens r and r + 8 are the k-slots of two products, Q's registers hold the
+// same values; the 16 bytes of V at value 64 i + 8 r of tokens 2c, 2c + 1,
+// 2c + 8 and 2c + 9 are column r of the eight products (i, e), column n of
+// which is value 64 i + 8 n + e.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kWarps * 32) scored_split_kernel(const ScoredArgs a, const ScoredPlan pl, int blocks) {
-  constexpr int NK = D / 32;
-  extern __shared__ float sm[];
+__global__ void __launch_bounds__(kWarps * 32, kResident)
+    scored_split_kernel(const ScoredArgs a, const ScoredPlan pl) {
+  constexpr int NK = D / 32, RB = ROWS / 8;
+  __shared__ uint4 q_sm[kWarps][RB][NK][32];
   ptx::pdl_launch_dependents();
   ptx::pdl_wait();
-  const int req = blockIdx.z, h = blockIdx.y;
-  const int ch = blockIdx.x / blocks, rb = blockIdx.x % blocks;
-  const int cap = min(a.max_len, (int)min((long long)a.bt_pages * a.page_size, 0x7fffffffll));
-  const int n = checked_len(a.kv_lens[req], cap, a.status, kSiteScoredLen, blockIdx.x == 0 && h == 0 && threadIdx.x == 0);
-  const int t0 = ch * pl.chunk;
-  if (t0 >= n) return;
-  const int t1 = min(n, t0 + pl.chunk);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
-  const int G = a.Hq / a.Hkv, row0 = rb * ROWS;
-  const int n_rows = min(ROWS, pl.rows - row0);
+  const int cap = table_cap(a.max_len, a.bt_pages, a.page_size);
+  const int G = a.Hq / a.Hkv, HB = a.Hkv * pl.blocks;
+  const uint32_t w_id = blockIdx.x * kWarps + warp;
+  auto tiles_of = [&](int n) { return (n + kTile - 1) / kTile; };
 
-  // this lane's query rows r and r + 8: operand registers and token limits
-  uint4 qx[ROWS / 8][NK];
-  int lim[ROWS / 8];
+  // this warp's run of the list (its length fits 31 bits)
+  uint32_t total = 0;
+  for (int i = lane; i < a.R; i += 32) total += tiles_of(checked_len(a.kv_lens[i], cap, a.status, kSiteScoredLen, w_id == 0));
+  total = __reduce_add_sync(0xffffffffu, total) * HB;
+  const uint32_t per = run_length(total, gridDim.x * kWarps);
+  if ((unsigned long long)w_id * per >= total) return;
+  const uint32_t u0 = w_id * per;
+  uint32_t left = min(per, total - u0);
+  int req = 0, hb = 0, tile = 0;
+  {
+    uint32_t before = 0;  // tiles (of one head) in front of request i0
+    for (int i0 = 0;; i0 += 32) {
+      const uint32_t own = i0 + lane < a.R ? tiles_of(checked_len(a.kv_lens[i0 + lane], cap, nullptr, 0, false)) : 0;
+      uint32_t inc = own;
 #pragma unroll
-  for (int i = 0; i < ROWS / 8; ++i) {
-    const int row = row0 + r + 8 * i;
-    lim[i] = 0;
-#pragma unroll
-    for (int kk = 0; kk < NK; ++kk) qx[i][kk] = make_uint4(0, 0, 0, 0);
-    if (row < pl.rows) {
-      const int qi = row / G, g = row - qi * G;
-      lim[i] = n - (a.Q - 1 - qi);
-      const T *src = static_cast<const T *>(a.q) + (size_t)req * a.q_req + (size_t)qi * a.q_query +
-                     (size_t)(h * G + g) * D + c * 8;
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) qx[i][kk] = *reinterpret_cast<const uint4 *>(src + kk * 32);
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, (before + inc) * HB > u0);
+      if (past != 0u) {
+        const int at = __ffs(past) - 1;
+        const uint32_t off = u0 - (before + __shfl_sync(0xffffffffu, inc - own, at)) * HB;
+        const uint32_t nt = __shfl_sync(0xffffffffu, own, at);
+        req = i0 + at;
+        hb = (int)(off / nt);
+        tile = (int)(off - (uint32_t)hb * nt);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
     }
   }
-  // tokens below all_see are seen by every row of this block
-  const int all_see = n - (a.Q - 1 - row0 / G);
+  int n = checked_len(a.kv_lens[req], cap, nullptr, 0, false);
+
+  int lim[RB], all_see = 0;  // tokens that rows r, r + 8 see; tokens that every row of the task sees
   const float scale2 = a.sm_scale * kLog2e;
-  const int32_t *bt = a.block_table + (size_t)req * a.bt_stride;
-  float *s_out = a.ws + pl.s_off + ((size_t)req * a.Hkv + h) * pl.rows * pl.lp;
-
-  float o[D / 8][ROWS / 4];
+  float *s_out = nullptr;
+  auto enter_task = [&]() {
+    const int h = hb / pl.blocks, row0 = (hb - h * pl.blocks) * ROWS;
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i)
+    for (int i = 0; i < RB; ++i) {
+      const int row = row0 + r + 8 * i;
+      lim[i] = 0;
+      const T *src = nullptr;
+      if (row < pl.rows) {
+        const int qi = row / G, g = row - qi * G;
+        lim[i] = n - (a.Q - 1 - qi);
+        src = static_cast<const T *>(a.q) + (size_t)req * a.q_req + (size_t)qi * a.q_query + (size_t)(h * G + g) * D + c * 8;
+      }
 #pragma unroll
-    for (int j = 0; j < ROWS / 4; ++j) o[i][j] = 0.f;
-  float m[ROWS / 8], sum[ROWS / 8];
-#pragma unroll
-  for (int i = 0; i < ROWS / 8; ++i) m[i] = -INFINITY, sum[i] = 0.f;
-
+      for (int kk = 0; kk < NK; ++kk)  // each lane reads back only what it wrote
+        q_sm[warp][i][kk][lane] = src != nullptr ? *reinterpret_cast<const uint4 *>(src + kk * 32) : make_uint4(0, 0, 0, 0);
+    }
+    all_see = n - (a.Q - 1 - row0 / G);
+    s_out = a.ws + pl.s_off + ((size_t)req * a.Hkv + h) * pl.rows * pl.lp + (size_t)(row0 + r) * pl.lp + 2 * c;
+  };
   // first element of a tile's K rows, or a negative number for a bad page
-  auto tile_row = [&](int tok) -> long long {
-    const int col = tok / a.page_size;
-    const int page = bt[col];
+  auto tile_row = [&](int q, int hb_, int t) -> long long {
+    const int tok = t * kTile, col = tok / a.page_size;
+    const int page = a.block_table[(size_t)q * a.bt_stride + col];
     if (page < 0 || page >= a.num_pages) {
-      if (lane == 0 && rb == 0) report_bad_index(a.status, kSiteScoredPage, page);
+      if (lane == 0) report_bad_index(a.status, kSiteScoredPage, page);
       return -1;
     }
-    return (((long long)page * a.Hkv + h) * a.page_size + (tok - col * a.page_size)) * D;
+    return (((long long)page * a.Hkv + hb_ / pl.blocks) * a.page_size + (tok - col * a.page_size)) * D;
   };
   uint4 kx[2][NK], vx[D / 64][4];
   auto load_k = [&](long long base) {
@@ -337,44 +356,68 @@ __global__ void __launch_bounds__(kWarps * 32) scored_split_kernel(const ScoredA
       for (int kk = 0; kk < NK; ++kk) kx[j][kk] = ld_stream(p + j * 8 * D + kk * 32);
   };
   auto load_v = [&](long long base) {
-    const T *p = static_cast<const T *>(a.v_cache) + (base < 0 ? 0 : base) + r * 8;
+    const T *p = static_cast<const T *>(a.v_cache) + (base < 0 ? 0 : base) + 2 * c * D + r * 8;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      vx[i][0] = ld_stream(p + (2 * c) * D + i * 64);
-      vx[i][1] = ld_stream(p + (2 * c + 1) * D + i * 64);
-      vx[i][2] = ld_stream(p + (2 * c + 8) * D + i * 64);
-      vx[i][3] = ld_stream(p + (2 * c + 9) * D + i * 64);
-    }
+    for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) vx[i][j] = ld_stream(p + ((j & 1) + (j / 2) * 8) * D + i * 64);
   };
 
-  int tok = t0 + warp * kTile;
-  long long base = -1;
-  if (tok < t1) {
-    base = tile_row(tok);
-    load_k(base);
-    load_v(base);
-  }
-  for (; tok < t1; tok += kWarps * kTile) {
-    const int next = tok + kWarps * kTile;
-    const long long next_base = next < t1 ? tile_row(next) : -1;
+  float o[D / 8][ROWS / 4];
+  float m[RB], sum[RB];
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < ROWS / 4; ++j) o[i][j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < RB; ++i) m[i] = -INFINITY, sum[i] = 0.f;
+  };
+
+  long long base = tile_row(req, hb, tile);
+  load_k(base);
+  load_v(base);
+  enter_task();
+  clear();
+  int nt = tiles_of(n);
+  while (true) {
+    --left;
+    int n_req = req, n_hb = hb, n_tile = tile + 1, n_n = n;
+    const bool task_ends = n_tile == nt || left == 0;
+    long long next = -1;
+    if (left > 0) {
+      if (n_tile == nt) {
+        n_tile = 0;
+        if (++n_hb == HB) {
+          n_hb = 0;
+          do n_n = checked_len(a.kv_lens[++n_req], cap, nullptr, 0, false);
+          while (n_n == 0);  // more tiles follow, so a request with some does
+        }
+      }
+      next = tile_row(n_req, n_hb, n_tile);
+    }
     float s[2][4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+    for (int j = 0; j < 2; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk) {
-        const uint4 q0 = qx[0][kk], q1 = ROWS == 16 ? qx[ROWS / 8 - 1][kk] : make_uint4(0, 0, 0, 0);
+    for (int kk = 0; kk < NK; ++kk) {
+      const uint4 q0 = q_sm[warp][0][kk][lane];
+      const uint4 q1 = ROWS == 16 ? q_sm[warp][RB - 1][kk][lane] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
         mma16816<T>(s[j][0], s[j][1], s[j][2], s[j][3], q0.x, q1.x, q0.y, q1.y, kx[j][kk].x, kx[j][kk].y);
         mma16816<T>(s[j][0], s[j][1], s[j][2], s[j][3], q0.z, q1.z, q0.w, q1.w, kx[j][kk].z, kx[j][kk].w);
       }
     }
-    if (next < t1) load_k(next_base);
+    if (left > 0) load_k(next);
     // tokens from `end` on are not there (behind the request's end, or their page is bad)
+    const int tok = tile * kTile;
     const int end = base < 0 ? tok : n;
     const bool whole = tok + kTile <= min(end, all_see);
     uint32_t pa[2][2] = {{0u, 0u}, {0u, 0u}};  // [row block][tile half]: P as the product's A operand
+    const int row0 = (hb % pl.blocks) * ROWS;
 #pragma unroll
-    for (int i = 0; i < ROWS / 8; ++i) {
+    for (int i = 0; i < RB; ++i) {
       float v[4] = {s[0][2 * i] * scale2, s[0][2 * i + 1] * scale2, s[1][2 * i] * scale2, s[1][2 * i + 1] * scale2};
       if (!whole) {
         const int seen = min(end, lim[i]);
@@ -382,9 +425,8 @@ __global__ void __launch_bounds__(kWarps * 32) scored_split_kernel(const ScoredA
         for (int j = 0; j < 4; ++j)
           if (tok + (j / 2) * 8 + 2 * c + (j & 1) >= seen) v[j] = -INFINITY;
       }
-      const int row = row0 + r + 8 * i;
-      if (row < pl.rows) {
-        float *dst = s_out + (size_t)row * pl.lp + tok + 2 * c;
+      if (row0 + r + 8 * i < pl.rows) {
+        float *dst = s_out + (size_t)(8 * i) * pl.lp + tok;
         *reinterpret_cast<float2 *>(dst) = make_float2(v[0], v[1]);
         *reinterpret_cast<float2 *>(dst + 8) = make_float2(v[2], v[3]);
       }
@@ -408,20 +450,15 @@ __global__ void __launch_bounds__(kWarps * 32) scored_split_kernel(const ScoredA
       pa[i][1] = pack2<T>(v[2], v[3]);
     }
     if (tok + kTile > end) {  // 0 * NaN: values behind the end must not reach the product
-      const bool k0 = tok + 2 * c < end, k1 = tok + 2 * c + 1 < end, k2 = tok + 2 * c + 8 < end, k3 = tok + 2 * c + 9 < end;
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) {
-        vx[i][0] = keep_if(k0, vx[i][0]);
-        vx[i][1] = keep_if(k1, vx[i][1]);
-        vx[i][2] = keep_if(k2, vx[i][2]);
-        vx[i][3] = keep_if(k3, vx[i][3]);
-      }
+      for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vx[i][j] = keep_if(tok + (j / 2) * 8 + 2 * c + (j & 1) < end, vx[i][j]);
     }
     bool apart = false;
     if (a.Q > 1 && tok + kTile > all_see) {
-      // tokens that only the later queries see: if one holds an infinity or
-      // a NaN, the queries are added one at a time, each without the tokens
-      // that it does not see
+      // tokens that only the later queries see: an infinity or a NaN among
+      // them must not meet the zero weight of a query that does not
       bool odd = false;
 #pragma unroll
       for (int i = 0; i < D / 64; ++i)
@@ -435,69 +472,74 @@ __global__ void __launch_bounds__(kWarps * 32) scored_split_kernel(const ScoredA
       apart = __any_sync(0xffffffffu, odd);
     }
     if (!apart) {
-      add_pv<T, D, ROWS>(o, vx, pa[0][0], pa[1][0], pa[0][1], pa[1][1]);
-    } else {
-      for (int qi = row0 / G; qi <= (row0 + n_rows - 1) / G; ++qi) {
-        const int seen = min(end, n - (a.Q - 1 - qi));
-        uint4 vq[D / 64][4];
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i)
+      for (int i = 0; i < D / 64; ++i) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) vq[i][j] = keep_if(tok + (j / 2) * 8 + 2 * c + (j & 1) < seen, vx[i][j]);
-        const bool mine0 = (row0 + r) / G == qi, mine1 = (row0 + r + 8) / G == qi;
-        // rows of the other queries: 0 * NaN again, so their sums are put back
-        float old[D / 8][ROWS / 4];
+        for (int e = 0; e < 8; ++e) {
+          auto word = [&](int j) { return e / 2 == 0 ? vx[i][j].x : e / 2 == 1 ? vx[i][j].y : e / 2 == 2 ? vx[i][j].z : vx[i][j].w; };
+          const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
+          const uint32_t b0 = __byte_perm(word(0), word(1), sel), b1 = __byte_perm(word(2), word(3), sel);
+          float(&acc)[ROWS / 4] = o[i * 8 + e];
+          if constexpr (ROWS == 16) {
+            mma16816<T>(acc[0], acc[1], acc[2], acc[3], pa[0][0], pa[1][0], pa[0][1], pa[1][1], b0, b1);
+          } else {
+            float z0 = 0.f, z1 = 0.f;  // rows 8-15 of the product: unused
+            mma16816<T>(acc[0], acc[1], z0, z1, pa[0][0], 0u, pa[0][1], 0u, b0, b1);
+          }
+        }
+      }
+    } else {  // token by token, each row only with what it sees
+      for (int t = 0; t < kTile && tok + t < end; ++t) {
+        const T *src = static_cast<const T *>(a.v_cache) + base + t * D + 16 * c;
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d)
+        for (int i = 0; i < RB; ++i) {
+          const uint32_t two = __shfl_sync(0xffffffffu, t < 8 ? pa[i][0] : pa[i][1], r * 4 + (t & 7) / 2);
+          const float2 pp = unpack2<T>(two);
+          const float w = (t & 1) ? pp.y : pp.x;
+          if (tok + t < lim[i]) {
 #pragma unroll
-          for (int j = 0; j < ROWS / 4; ++j) old[d][j] = o[d][j];
-        add_pv<T, D, ROWS>(o, vq, pa[0][0], pa[1][0], pa[0][1], pa[1][1]);
+            for (int d = 0; d < D / 64; ++d) {
+              float lo[8], hi[8];
+              unpack8<T>(*reinterpret_cast<const uint4 *>(src + d * 64), lo);
+              unpack8<T>(*reinterpret_cast<const uint4 *>(src + d * 64 + 8), hi);
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d)
-#pragma unroll
-          for (int j = 0; j < ROWS / 4; ++j)
-            if (!(j < 2 ? mine0 : mine1)) o[d][j] = old[d][j];
+              for (int e = 0; e < 8; ++e) {
+                o[d * 8 + e][2 * i] += w * lo[e];
+                o[d * 8 + e][2 * i + 1] += w * hi[e];
+              }
+            }
+          }
+        }
       }
     }
-    if (next < t1) load_v(next_base);
-    base = next_base;
-  }
+    if (left > 0) load_v(next);
+    if (task_ends) {
+      const size_t part = (size_t)w_id + (uint32_t)req * HB + hb;
 #pragma unroll
-  for (int i = 0; i < ROWS / 8; ++i) {
-    sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-    sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-  }
-
-  // join the warps: shared memory holds [warp][ROWS] (max, sum) and [warp][ROWS][D]
-  float2 *ml = reinterpret_cast<float2 *>(sm);
-  float *os = sm + 2 * kWarps * ROWS;
+      for (int i = 0; i < RB; ++i) {
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+        const int row = r + 8 * i;
+        if (row0 + row < pl.rows) {
+          float *dst = a.ws + pl.o_off + (part * ROWS + row) * D + 16 * c;
 #pragma unroll
-  for (int i = 0; i < ROWS / 8; ++i) {
-    if (c == 0) ml[warp * ROWS + r + 8 * i] = make_float2(m[i], sum[i]);
-    float *dst = os + ((size_t)warp * ROWS + r + 8 * i) * D;
+          for (int d = 0; d < D / 64; ++d)
 #pragma unroll
-    for (int d = 0; d < D / 8; ++d) {
-      dst[(d / 8) * 64 + 16 * c + d % 8] = o[d][2 * i];
-      dst[(d / 8) * 64 + 16 * c + 8 + d % 8] = o[d][2 * i + 1];
+            for (int e = 0; e < 16; e += 4) {
+              const int x = d * 8 + e % 8, y = 2 * i + e / 8;
+              *reinterpret_cast<float4 *>(dst + d * 64 + e) = make_float4(o[x][y], o[x + 1][y], o[x + 2][y], o[x + 3][y]);
+            }
+          if (c == 0) reinterpret_cast<float2 *>(a.ws + pl.ml_off)[part * ROWS + row] = make_float2(m[i], sum[i]);
+        }
+      }
+      if (left == 0) return;
+      req = n_req, hb = n_hb, n = n_n;
+      nt = tiles_of(n);
+      enter_task();
+      clear();
     }
-  }
-  __syncthreads();
-  const size_t part = ((size_t)req * a.Hkv + h) * pl.nch + ch;
-  for (int x = threadIdx.x; x < n_rows * D; x += kWarps * 32) {
-    const int row = x / D;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w * ROWS + row].x);
-    float v = 0.f, tot = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = scale_to(ml[w * ROWS + row].x, top);
-      v += os[((size_t)w * ROWS + row) * D + x % D] * f;
-      tot += ml[w * ROWS + row].y * f;
-    }
-    const size_t at = part * pl.rows + row0 + row;
-    a.ws[pl.o_off + at * D + x % D] = v;
-    if (x % D == 0) reinterpret_cast<float2 *>(a.ws + pl.ml_off)[at] = make_float2(top, tot);
+    tile = n_tile;
+    base = next;
   }
 }
 
@@ -506,87 +548,177 @@ __device__ __forceinline__ void red_add4(float *p, const float4 &v) {
                : "memory");
 }
 
-// Join: every CTA of a request and KV head derives the rows' lse from the
-// chunks' (max, sum); each joins the outputs of some rows and adds the weights
-// of its own chunk's tokens. Rows are summed in a fixed order, and one
-// request's pages get one addition per token and head from a call.
+// Join. The first CTAs of a (request, KV head) join the outputs of two rows
+// each (four warps to a row, each a quarter of the partial results); the
+// others add the weights of pl.join tokens each: a thread has four tokens and
+// every groups-th row, whose logits it requests before the rows' lse is known.
+// All sums have a fixed order, and one request's pages get one addition per
+// token and head from a call.
+constexpr int kJoin = 256;
+constexpr int kJoinRows = 2;
+
+// Partial results of a task: first index and count.
+struct Parts {
+  uint32_t first, count;
+};
+__device__ __forceinline__ Parts parts_of(uint32_t before, uint32_t per, int nt, int HB, int req, int hb) {
+  const uint32_t u0 = before * HB + (uint32_t)hb * nt, w0 = u0 / per;
+  return {w0 + (uint32_t)req * HB + hb, nt == 0 ? 0u : (u0 + nt - 1) / per - w0 + 1};
+}
+// log2 of a row's sum over its partial results (NaN where a logit is), by the
+// LANES aligned lanes that share the row
+template <int LANES>
+__device__ __forceinline__ float row_lse2(const float2 *ml, uint32_t count, int pitch) {
+  const int lane = threadIdx.x % LANES;
+  float top = -INFINITY, tot = 0.f;
+#pragma unroll 4
+  for (uint32_t k = lane; k < count; k += LANES) {
+    const float2 v = ml[(size_t)k * pitch];
+    const float t = fmaxf(top, v.x);
+    tot = tot * scale_to(top, t) + v.y * scale_to(v.x, t);
+    top = t;
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    const float ot = __shfl_xor_sync(0xffffffffu, top, o), os = __shfl_xor_sync(0xffffffffu, tot, o);
+    const float t = fmaxf(top, ot);
+    tot = tot * scale_to(top, t) + os * scale_to(ot, t);
+    top = t;
+  }
+  return top == -INFINITY && tot == 0.f ? -INFINITY : top + log2f(tot);
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) scored_join_kernel(const ScoredArgs a, const ScoredPlan pl) {
-  extern __shared__ float sm[];
-  float *lse2 = sm;                 // [rows]: log2 of the sum; +inf for a row that sees nothing
-  float *part_o = sm + pl.rows;     // [256]
+__global__ void __launch_bounds__(kJoin) scored_join_kernel(const ScoredArgs a, const ScoredPlan pl, int o_ctas) {
+  extern __shared__ __align__(16) float sm[];
+  __shared__ uint32_t red[2][kJoin / 32];
   ptx::pdl_launch_dependents();
   ptx::pdl_wait();
-  const int req = blockIdx.z, h = blockIdx.y, ch = blockIdx.x;
-  const int cap = min(a.max_len, (int)min((long long)a.bt_pages * a.page_size, 0x7fffffffll));
+  const int req = blockIdx.z, h = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int cap = table_cap(a.max_len, a.bt_pages, a.page_size);
   const int n = checked_len(a.kv_lens[req], cap, nullptr, 0, false);
-  const int nce = (n + pl.chunk - 1) / pl.chunk;
-  if (ch >= max(nce, 1)) return;
-  const int G = a.Hq / a.Hkv;
-  const size_t part = ((size_t)req * a.Hkv + h) * pl.nch;
-  const float2 *ml = reinterpret_cast<const float2 *>(a.ws + pl.ml_off) + part * pl.rows;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  for (int row = warp; row < pl.rows; row += 8) {
-    float top = -INFINITY, tot = 0.f;
-    for (int k = lane; k < nce; k += 32) {
-      const float2 v = ml[(size_t)k * pl.rows + row];
-      const float t = fmaxf(top, v.x);
-      tot = tot * scale_to(top, t) + v.y * scale_to(v.x, t);
-      top = t;
-    }
+  const bool weigh = (int)blockIdx.x >= o_ctas;
+  const int t0 = ((int)blockIdx.x - o_ctas) * pl.join, t1 = min(n, t0 + pl.join);
+  if (weigh && t0 >= n) return;
+  const int G = a.Hq / a.Hkv, HB = a.Hkv * pl.blocks, nt = (n + kTile - 1) / kTile;
+
+  // this thread's first logits
+  constexpr int PRE = 4;
+  const int quads = min(pl.join / 4, kJoin), groups = kJoin / quads, grp = tid / quads, quad = tid % quads;
+  const float *s_in = a.ws + pl.s_off + ((size_t)req * a.Hkv + h) * pl.rows * pl.lp;
+  float4 pre[PRE];
+  if (weigh && t0 + quad * 4 < t1) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float ot = __shfl_xor_sync(0xffffffffu, top, o), os = __shfl_xor_sync(0xffffffffu, tot, o);
-      const float t = fmaxf(top, ot);
-      tot = tot * scale_to(top, t) + os * scale_to(ot, t);
-      top = t;
-    }
-    if (lane == 0) {
-      const float v = top == -INFINITY && tot == 0.f ? -INFINITY : top + log2f(tot);  // NaN logits stay NaN
-      lse2[row] = v == -INFINITY ? INFINITY : v;
-      if (ch == 0 && a.lse != nullptr) {
+    for (int j = 0; j < PRE; ++j)
+      if (grp + j * groups < pl.rows)
+        pre[j] = *reinterpret_cast<const float4 *>(s_in + (size_t)(grp + j * groups) * pl.lp + t0 + quad * 4);
+  }
+  uint32_t before = 0, total = 0;
+  for (int i = tid; i < a.R; i += kJoin) {
+    const uint32_t t = (uint32_t)(checked_len(a.kv_lens[i], cap, nullptr, 0, false) + kTile - 1) / kTile;
+    total += t;
+    if (i < req) before += t;
+  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  total = __reduce_add_sync(0xffffffffu, total);
+  if (lane == 0) red[0][warp] = before, red[1][warp] = total;
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int w = 0; w < kJoin / 32; ++w) before += red[0][w], total += red[1][w];
+  const uint32_t per = run_length(total * HB, (uint32_t)(pl.grid * kWarps));
+  const float2 *ml = reinterpret_cast<const float2 *>(a.ws + pl.ml_off);
+
+  if (!weigh) {
+    constexpr int SUB = kJoin / 32 / kJoinRows, V = D / 32;  // warps per row, values per lane
+    const int row = blockIdx.x * kJoinRows + warp / SUB, sub = warp % SUB;
+    float v[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = 0.f;
+    if (row < pl.rows) {
+      const Parts pt = parts_of(before, per, nt, HB, req, h * pl.blocks + row / pl.block);
+      const float2 *mr = ml + (size_t)pt.first * pl.block + row % pl.block;
+      const float lse2 = row_lse2<32>(mr, pt.count, pl.block);
+      const float ref = lse2 == -INFINITY ? INFINITY : lse2;
+      const float *src = a.ws + pl.o_off + ((size_t)pt.first * pl.block + row % pl.block) * D + lane * V;
+#pragma unroll 4
+      for (uint32_t k = sub; k < pt.count; k += SUB) {
+        const float f = ex2_approx(mr[(size_t)k * pl.block].x - ref);
+        float p[V];
+        if constexpr (V == 4)
+          *reinterpret_cast<float4 *>(p) = *reinterpret_cast<const float4 *>(src + (size_t)k * pl.block * D);
+        else
+          *reinterpret_cast<float2 *>(p) = *reinterpret_cast<const float2 *>(src + (size_t)k * pl.block * D);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] += f != 0.f ? p[e] * f : 0.f;
+      }
+      if (sub == 0 && lane == 0 && a.lse != nullptr) {
         const int qi = row / G;
-        a.lse[((size_t)req * a.Q + qi) * a.Hq + h * G + (row - qi * G)] = v * kLn2;
+        a.lse[((size_t)req * a.Q + qi) * a.Hq + h * G + (row - qi * G)] = lse2 * kLn2;
       }
     }
+#pragma unroll
+    for (int e = 0; e < V; ++e) sm[warp * D + lane * V + e] = v[e];
+    __syncthreads();
+    if (row < pl.rows && sub == 0) {
+      const int qi = row / G;
+      T *dst = static_cast<T *>(a.out) + (size_t)req * a.out_req + (size_t)qi * a.out_query + (size_t)(h * G + row - qi * G) * D;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+#pragma unroll
+        for (int w = 1; w < SUB; ++w) v[e] += sm[(warp + w) * D + lane * V + e];
+        dst[lane * V + e] = narrow<T>(v[e]);
+      }
+    }
+    return;
+  }
+
+  float4 *part_w = reinterpret_cast<float4 *>(sm);  // [kJoin]
+  float *lse2 = sm + 4 * kJoin;                     // [rows]: +inf for a row that sees nothing
+  constexpr int LR = 8;                             // lanes per row
+  for (int row = tid / LR; row - tid / LR < pl.rows; row += kJoin / LR) {
+    const bool in = row < pl.rows;
+    const Parts pt = parts_of(before, per, nt, HB, req, h * pl.blocks + (in ? row : 0) / pl.block);
+    const float v = row_lse2<LR>(ml + (size_t)pt.first * pl.block + (in ? row : 0) % pl.block, pt.count, pl.block);
+    if (in && tid % LR == 0) lse2[row] = v == -INFINITY ? INFINITY : v;
   }
   __syncthreads();
-  const float *o_in = a.ws + pl.o_off + part * pl.rows * D;
-  constexpr int GR = 256 / D;
-  const int grp = threadIdx.x / D, d = threadIdx.x % D;
-  for (int row = ch; row < pl.rows; row += max(nce, 1)) {
-    const float ref = lse2[row];
-    float v = 0.f;
-#pragma unroll 4
-    for (int k = grp; k < nce; k += GR) {
-      const float f = ex2_approx(ml[(size_t)k * pl.rows + row].x - ref);
-      if (f != 0.f) v += o_in[((size_t)k * pl.rows + row) * D + d] * f;
-    }
-    part_o[threadIdx.x] = v;
-    __syncthreads();
-    if (grp == 0) {
-#pragma unroll
-      for (int k = 1; k < GR; ++k) v += part_o[k * D + d];
-      const int qi = row / G;
-      static_cast<T *>(a.out)[(size_t)req * a.out_req + (size_t)qi * a.out_query + (size_t)(h * G + row - qi * G) * D + d] =
-          narrow<T>(v);
-    }
-    __syncthreads();
-  }
-  const int t0 = ch * pl.chunk, t1 = min(n, t0 + pl.chunk);
-  const float *s_in = a.ws + pl.s_off + ((size_t)req * a.Hkv + h) * pl.rows * pl.lp;
-  const int32_t *bt = a.block_table + (size_t)req * a.bt_stride;
-  for (int tok = t0 + threadIdx.x * 4; tok < t1; tok += 1024) {
+  for (int tq = t0; tq < t1; tq += quads * 4) {
+    const int tok = tq + quad * 4;
     float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int row = 0; row < pl.rows; ++row) {
-      const float4 s = *reinterpret_cast<const float4 *>(s_in + (size_t)row * pl.lp + tok);
-      const float ref = lse2[row];
+    auto add = [&](const float4 &s, float ref) {
       w.x += ex2_approx(s.x - ref);
       w.y += ex2_approx(s.y - ref);
       w.z += ex2_approx(s.z - ref);
       w.w += ex2_approx(s.w - ref);
+    };
+    if (tok < t1) {
+#pragma unroll
+      for (int j = 0; j < PRE; ++j)
+        if (grp + j * groups < pl.rows) add(pre[j], lse2[grp + j * groups]);
+#pragma unroll 4
+      for (int row = grp + PRE * groups; row < pl.rows; row += groups)
+        add(*reinterpret_cast<const float4 *>(s_in + (size_t)row * pl.lp + tok), lse2[row]);
     }
-    const int col = tok / a.page_size, page = bt[col];
+    if (tok + quads * 4 < t1) {
+#pragma unroll
+      for (int j = 0; j < PRE; ++j)
+        if (grp + j * groups < pl.rows)
+          pre[j] = *reinterpret_cast<const float4 *>(s_in + (size_t)(grp + j * groups) * pl.lp + tok + quads * 4);
+    }
+    if (groups > 1) {
+      part_w[tid] = w;
+      __syncthreads();
+      if (grp == 0)
+        for (int k = 1; k < groups; ++k) {
+          const float4 p = part_w[k * quads + quad];
+          w.x += p.x, w.y += p.y, w.z += p.z, w.w += p.w;
+        }
+      __syncthreads();
+    }
+    if (grp != 0 || tok >= t1) continue;
+    const int col = tok / a.page_size, page = a.block_table[(size_t)req * a.bt_stride + col];
     if (page < 0 || page >= a.num_pages) continue;  // reported by the split kernel
     float *dst = a.scores + ((size_t)page * a.Hkv + h) * a.page_size + (tok - col * a.page_size);
     if (tok + 4 <= t1) {
@@ -832,16 +964,12 @@ extern "C" long long sched_attn_scored_ws_floats(int R, int Q, int Hq, int Hkv, 
 namespace kvb {
 template <typename T, int D>
 int run_scored(const ScoredArgs &a, const ScoredPlan &pl, cudaStream_t st) {
-  const bool small = pl.rows <= 8;
-  const int per = small ? 8 : 16, blocks = (pl.rows + per - 1) / per;
-  const size_t smem = (size_t)kWarps * per * (D + 2) * sizeof(float);
-  const long long gx = (long long)pl.nch * blocks;
-  if (gx > 0x7fffffffll) return -1;
-  auto *split = small ? scored_split_kernel<T, D, 8> : scored_split_kernel<T, D, 16>;
-  launch_pdl(split, dim3((unsigned)gx, a.Hkv, a.R), dim3(kWarps * 32), smem, st, a, pl, blocks);
+  auto *split = pl.block == 8 ? scored_split_kernel<T, D, 8> : scored_split_kernel<T, D, 16>;
+  launch_pdl(split, dim3(pl.grid), dim3(kWarps * 32), 0, st, a, pl);
   if (cudaPeekAtLastError() != cudaSuccess) return -4;
-  launch_pdl(scored_join_kernel<T, D>, dim3(pl.nch, a.Hkv, a.R), dim3(256), (size_t)(pl.rows + 256) * sizeof(float), st,
-             a, pl);
+  const int o_ctas = (pl.rows + kJoinRows - 1) / kJoinRows;
+  launch_pdl(scored_join_kernel<T, D>, dim3(o_ctas + (a.max_len + pl.join - 1) / pl.join, a.Hkv, a.R),
+             dim3(kJoin), (size_t)(pl.rows + 4 * kJoin) * sizeof(float), st, a, pl, o_ctas);
   return launched();
 }
 }  // namespace kvb
@@ -857,6 +985,8 @@ extern "C" int sched_attn_scored(const ScoredArgs *args, cudaStream_t st) {
       !aligned16(a.scores) || !aligned16(a.ws))
     return -1;
   const kvb::ScoredPlan pl = kvb::scored_plan(a.R, a.Q, a.Hq, a.Hkv, a.D, a.max_len, a.num_sms);
+  // the tile list is indexed in 32 bits (2^31 tiles are 2^35 cached tokens and heads)
+  if ((long long)a.R * a.Hkv * pl.blocks * (pl.lp / kvb::kTile) > 0x7fffffffll) return -1;
   if (a.ws == nullptr || a.ws_floats < pl.total) return -2;
   if (a.element == kKvFp16)
     return a.D == 128 ? kvb::run_scored<__half, 128>(a, pl, st) : kvb::run_scored<__half, 64>(a, pl, st);
