@@ -821,7 +821,7 @@ void qk_norm_rope_kv_append(const at::Tensor &qkv, const at::Tensor &wq, const a
   check_rc(rc_, "qk_norm_rope_kv_append");
 }
 
-// q, out [R, Q, Hq, D]; lse [R, Q, Hq]
+// q, out [R, Q, Hq, D] and lse [R, Q, Hq], or without Q for one query
 void attn_decode_scored(const at::Tensor &q, at::Tensor &out, const at::Tensor &k_cache, const at::Tensor &v_cache,
                         const at::Tensor &block_table, const at::Tensor &kv_lens, double sm_scale, at::Tensor &scores,
                         const c10::optional<at::Tensor> &lse, int64_t max_len, const c10::optional<at::Tensor> &status) {
@@ -830,24 +830,27 @@ void attn_decode_scored(const at::Tensor &q, at::Tensor &out, const at::Tensor &
   TORCH_CHECK(ps % 16 == 0, "the page size must be a multiple of 16");
   check_same(q, k_cache, "q");
   check_same(out, k_cache, "out");
-  TORCH_CHECK(q.dim() == 4 && q.size(3) == D && q.size(2) >= 1 && q.size(2) % Hkv == 0,
-              "q must be [requests, queries, q heads, head dim] with q heads a multiple of the cache's heads");
+  const int64_t nd = q.dim();
+  TORCH_CHECK((nd == 3 || nd == 4) && q.size(-1) == D && q.size(-2) >= 1 && q.size(-2) % Hkv == 0,
+              "q must be [requests, (queries,) q heads, head dim] with q heads a multiple of the cache's heads");
   TORCH_CHECK(out.sizes() == q.sizes(), "out must have q's shape");
-  const int64_t R = q.size(0), Q = q.size(1), Hq = q.size(2);
+  const int64_t R = q.size(0), Q = nd == 4 ? q.size(1) : 1, Hq = q.size(-2);
   for (const at::Tensor *t : {&q, (const at::Tensor *)&out})
-    TORCH_CHECK(t->numel() == 0 || (t->stride(3) == 1 && (t->stride(2) == D || Hq == 1) &&
+    TORCH_CHECK(t->numel() == 0 || (t->stride(-1) == 1 && (t->stride(-2) == D || Hq == 1) &&
                                     (Q == 1 || t->stride(1) % 8 == 0) && (R == 1 || t->stride(0) % 8 == 0)),
                 "q and out need contiguous heads and rows on 16-byte boundaries");
-  TORCH_CHECK(out.numel() == 0 || ((Q == 1 || out.stride(1) >= Hq * D) && (R == 1 || out.stride(0) >= Hq * D)),
+  TORCH_CHECK(out.numel() == 0 || ((Q == 1 || out.stride(1) >= Hq * D) && (R == 1 || out.stride(0) >= Hq * D) &&
+                                   (Q == 1 || R == 1 || out.stride(0) >= Q * out.stride(1) ||
+                                    out.stride(1) >= R * out.stride(0))),
               "rows of out must not overlap");
   TORCH_CHECK(R <= 65535 && Q * (Hq / Hkv) <= 8192, "at most 65535 requests and 8192 query rows per KV head");
   check_table(block_table, R);
   check_vec(kv_lens, at::kInt, R, "kv_lens", "int32");
   check_track(scores, k_cache, at::kFloat, "scores", "float32");
   if (lse.has_value()) {
-    TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->dim() == 3 && lse->size(0) == R &&
-                    lse->size(1) == Q && lse->size(2) == Hq,
-                "lse must be contiguous float32 [requests, queries, q heads]");
+    TORCH_CHECK(lse->scalar_type() == at::kFloat && lse->is_contiguous() && lse->dim() == nd - 1 && lse->size(0) == R &&
+                    (nd == 3 || lse->size(1) == Q) && lse->size(-1) == Hq,
+                "lse must be contiguous float32 of q's shape without the head dim");
   }
   TORCH_CHECK(max_len >= 0, "max_len must not be negative");
   int64_t cap = block_table.size(1) * ps;
@@ -860,6 +863,7 @@ void attn_decode_scored(const at::Tensor &q, at::Tensor &out, const at::Tensor &
   if (lse.has_value()) check_on(*lse, k_cache, "lse");
   if (R == 0 || Q == 0) return;
   check_aligned(q, "q");
+  check_aligned(out, "out");
   check_aligned(k_cache, "k_cache");
   check_aligned(v_cache, "v_cache");
   check_aligned(scores, "scores");
@@ -895,8 +899,9 @@ void attn_decode_scored(const at::Tensor &q, at::Tensor &out, const at::Tensor &
     c10::cuda::CUDAGuard g(k_cache.device());
     // scratch of this call alone, from the allocator's pool of the current stream (or of the graph being captured)
     const long long floats = sched_attn_scored_ws_floats(a.R, a.Q, a.Hq, a.Hkv, a.D, a.max_len, a.num_sms);
-    at::Tensor ws = at::empty({floats}, scores.options());
-    a.ws = ws.data_ptr<float>();
+    at::Tensor ws;
+    if (floats > 0) ws = at::empty({floats}, scores.options());
+    a.ws = floats > 0 ? ws.data_ptr<float>() : nullptr;
     a.ws_floats = floats;
     rc_ = sched_attn_scored(&a, cur_stream());
   }
@@ -961,8 +966,9 @@ void kv_evict(at::Tensor &k_cache, at::Tensor &v_cache, at::Tensor &scores, at::
   int rc_ = 0;
   {  // the guard is gone before check_rc may throw
     c10::cuda::CUDAGuard g(k_cache.device());
-    const long long ints = sched_kv_evict_ws_ints(a.R, a.Hkv, a.max_len, a.budget);
-    at::Tensor ws = at::empty({ints}, kv_lens.options());
+    const long long ints = sched_kv_evict_ws_ints(a.R, a.Hkv, a.max_len, a.budget, a.num_sms);
+    at::Tensor ws;
+    if (ints > 0) ws = at::empty({ints}, kv_lens.options());
     a.ws = ints > 0 ? ws.data_ptr<int32_t>() : nullptr;
     a.ws_ints = ints;
     rc_ = sched_kv_evict(&a, cur_stream());

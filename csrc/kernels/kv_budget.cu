@@ -181,8 +181,11 @@ constexpr int kMinRun = 2;     // tiles per warp at least: bounds the partial re
 struct ScoredPlan {
   int rows, lp;         // query rows per KV head, padded length
   int block, blocks;    // rows per task (8 or 16), tasks per (request, KV head)
-  int grid, join;       // CTAs of the split kernel, tokens per CTA of the join
-  long long s_off, o_off, ml_off, total;
+  int grid;             // CTAs of the split kernel
+  int join, o_rows;     // tokens per weight CTA and rows per output CTA of the join
+  // workspace: logits [R, Hkv, rows, lp], partial outputs and (max, sum) [parts, block],
+  // and for the join: tiles per warp, then (length, tiles in front) of each request
+  long long s_off, o_off, ml_off, meta_off, total;
 };
 
 inline ScoredPlan scored_plan(int R, int Q, int Hq, int Hkv, int D, int max_len, int num_sms) {
@@ -195,13 +198,19 @@ inline ScoredPlan scored_plan(int R, int Q, int Hq, int Hkv, int D, int max_len,
   const long long most = (tasks * (p.lp / kTile) + kMinRun * kWarps - 1) / (kMinRun * kWarps);
   const long long fill = (long long)num_sms * kResident;
   p.grid = (int)(most < fill ? most : fill);
-  p.join = 2048;
-  while (p.join > 256 && heads * ((max_len + p.join - 1) / p.join) < num_sms) p.join /= 2;
+  // the join's CTAs all resident at once where that is possible, with each thread having a logit to read
+  p.join = p.rows >= 16 ? 64 : p.rows >= 8 ? 128 : p.rows >= 4 ? 256 : p.rows >= 2 ? 512 : 1024;
+  while (heads * ((max_len + p.join - 1) / p.join) > 3ll * num_sms && p.join < max_len) p.join += p.join < 1024 ? p.join : 1024;
+  // and at most 16 partial results per warp
+  p.o_rows = 1;
+  while (p.o_rows < 8 && heads * ((p.rows + p.o_rows - 1) / p.o_rows) > num_sms && p.grid * kWarps / tasks * p.o_rows * 2 <= 8 * 16)
+    p.o_rows *= 2;
   p.s_off = 0;
   p.o_off = heads * p.rows * p.lp;
   const long long parts = (long long)p.grid * kWarps + tasks;
   p.ml_off = p.o_off + parts * p.block * D;
-  p.total = p.ml_off + parts * p.block * 2;
+  p.meta_off = p.ml_off + parts * p.block * 2;
+  p.total = p.meta_off + 1 + 2ll * R;
   return p;
 }
 
@@ -224,11 +233,12 @@ __device__ __forceinline__ void mma16816<__half>(float &d0, float &d1, float &d2
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint4 ld_stream(const void *p) {  // read once: not kept in L1
+// read once: not kept in L1, and the first to leave L2 (which the logits should not)
+__device__ __forceinline__ uint4 ld_stream(const void *p, uint64_t policy) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+               : "l"(p), "l"(policy));
   return v;
 }
 
@@ -255,13 +265,25 @@ __device__ __forceinline__ uint32_t run_length(uint32_t total, uint32_t warps) {
 
 __device__ __forceinline__ uint4 keep_if(bool k, const uint4 &v) { return k ? v : make_uint4(0, 0, 0, 0); }
 
-// One warp: a run of tiles. K and V go from global memory straight into the
-// registers of the m16n8k16 operands (K of the next tile is requested once
-// this one's logits are done, V once its product is), so a warp always has
-// loads in flight and there is no shared-memory staging; Q waits in shared
-// memory in operand order. Query rows are the M side (8 of its 16 rows where
-// a KV head has at most 8 query rows), tokens the N side of the logits and
-// the K side of the output.
+// First element of a tile's K (and V) rows, or a negative number for a bad page.
+__device__ __forceinline__ long long page_base(const ScoredArgs &a, int page, int h, int tok) {
+  if (page < 0 || page >= a.num_pages) {
+    if (threadIdx.x % 32 == 0) report_bad_index(a.status, kSiteScoredPage, page);
+    return -1;
+  }
+  return (((long long)page * a.Hkv + h) * a.page_size + tok % a.page_size) * a.D;
+}
+__device__ __forceinline__ long long tile_base(const ScoredArgs &a, int req, int h, int tok) {
+  return page_base(a, a.block_table[(size_t)req * a.bt_stride + tok / a.page_size], h, tok);
+}
+
+// A warp's running softmax over 16-token tiles. K and V go from global memory
+// straight into the registers of the m16n8k16 operands (K of the next tile is
+// requested once this one's logits are done, V once its product is), so a warp
+// always has loads in flight and there is no shared-memory staging; Q waits in
+// shared memory in operand order. Query rows are the M side (8 of its 16 rows
+// where a KV head has at most 8 query rows), tokens the N side of the logits
+// and the K side of the output.
 //
 // Operand layout, for lane 4 r + c: the 16 bytes of K at value 32 kk + 8 c of
 // tokens r and r + 8 are the k-slots of two products, Q's registers hold the
@@ -269,153 +291,82 @@ __device__ __forceinline__ uint4 keep_if(bool k, const uint4 &v) { return k ? v 
 // 2c + 8 and 2c + 9 are column r of the eight products (i, e), column n of
 // which is value 64 i + 8 n + e.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kWarps * 32, kResident)
-    scored_split_kernel(const ScoredArgs a, const ScoredPlan pl) {
-  constexpr int NK = D / 32, RB = ROWS / 8;
-  __shared__ uint4 q_sm[kWarps][RB][NK][32];
-  ptx::pdl_launch_dependents();
-  ptx::pdl_wait();
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
-  const int cap = table_cap(a.max_len, a.bt_pages, a.page_size);
-  const int G = a.Hq / a.Hkv, HB = a.Hkv * pl.blocks;
-  const uint32_t w_id = blockIdx.x * kWarps + warp;
-  auto tiles_of = [&](int n) { return (n + kTile - 1) / kTile; };
+struct RowSoftmax {
+  static constexpr int NK = D / 32, RB = ROWS / 8;
+  typedef uint4 QTile[RB][NK][32];  // each lane reads back only what it wrote
+  int lane, r, c;
+  uint4 kx[2][NK], vx[D / 64][4];
+  float o[D / 8][ROWS / 4];  // product (i, e) = o[8 i + e]: row r's columns 2c, 2c + 1, then row r + 8's
+  float m[RB], sum[RB];      // of rows r, r + 8; sum: this lane's tokens only, until finish()
+  int lim[RB], all_see;      // tokens that rows r, r + 8 see; tokens that every row of the task sees
+  int rows_here;             // rows of the task
+  uint64_t policy;
 
-  // this warp's run of the list (its length fits 31 bits)
-  uint32_t total = 0;
-  for (int i = lane; i < a.R; i += 32) total += tiles_of(checked_len(a.kv_lens[i], cap, a.status, kSiteScoredLen, w_id == 0));
-  total = __reduce_add_sync(0xffffffffu, total) * HB;
-  const uint32_t per = run_length(total, gridDim.x * kWarps);
-  if ((unsigned long long)w_id * per >= total) return;
-  const uint32_t u0 = w_id * per;
-  uint32_t left = min(per, total - u0);
-  int req = 0, hb = 0, tile = 0;
-  {
-    uint32_t before = 0;  // tiles (of one head) in front of request i0
-    for (int i0 = 0;; i0 += 32) {
-      const uint32_t own = i0 + lane < a.R ? tiles_of(checked_len(a.kv_lens[i0 + lane], cap, nullptr, 0, false)) : 0;
-      uint32_t inc = own;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, (before + inc) * HB > u0);
-      if (past != 0u) {
-        const int at = __ffs(past) - 1;
-        const uint32_t off = u0 - (before + __shfl_sync(0xffffffffu, inc - own, at)) * HB;
-        const uint32_t nt = __shfl_sync(0xffffffffu, own, at);
-        req = i0 + at;
-        hb = (int)(off / nt);
-        tile = (int)(off - (uint32_t)hb * nt);
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, inc, 31);
-    }
-  }
-  int n = checked_len(a.kv_lens[req], cap, nullptr, 0, false);
+  __device__ __forceinline__ RowSoftmax() : lane(threadIdx.x % 32), r(lane / 4), c(lane % 4), policy(ptx::policy_evict_first()) {}
 
-  int lim[RB], all_see = 0;  // tokens that rows r, r + 8 see; tokens that every row of the task sees
-  const float scale2 = a.sm_scale * kLog2e;
-  float *s_out = nullptr;
-  auto enter_task = [&]() {
-    const int h = hb / pl.blocks, row0 = (hb - h * pl.blocks) * ROWS;
+  __device__ __forceinline__ void enter(const ScoredArgs &a, int rows, int req, int h, int row0, int n, QTile &q_sm) {
+    const int G = a.Hq / a.Hkv;
+    rows_here = min(ROWS, rows - row0);
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
       const int row = row0 + r + 8 * i;
       lim[i] = 0;
       const T *src = nullptr;
-      if (row < pl.rows) {
+      if (row < rows) {
         const int qi = row / G, g = row - qi * G;
         lim[i] = n - (a.Q - 1 - qi);
         src = static_cast<const T *>(a.q) + (size_t)req * a.q_req + (size_t)qi * a.q_query + (size_t)(h * G + g) * D + c * 8;
       }
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk)  // each lane reads back only what it wrote
-        q_sm[warp][i][kk][lane] = src != nullptr ? *reinterpret_cast<const uint4 *>(src + kk * 32) : make_uint4(0, 0, 0, 0);
+      for (int kk = 0; kk < NK; ++kk)
+        q_sm[i][kk][lane] = src != nullptr ? *reinterpret_cast<const uint4 *>(src + kk * 32) : make_uint4(0, 0, 0, 0);
     }
     all_see = n - (a.Q - 1 - row0 / G);
-    s_out = a.ws + pl.s_off + ((size_t)req * a.Hkv + h) * pl.rows * pl.lp + (size_t)(row0 + r) * pl.lp + 2 * c;
-  };
-  // first element of a tile's K rows, or a negative number for a bad page
-  auto tile_row = [&](int q, int hb_, int t) -> long long {
-    const int tok = t * kTile, col = tok / a.page_size;
-    const int page = a.block_table[(size_t)q * a.bt_stride + col];
-    if (page < 0 || page >= a.num_pages) {
-      if (lane == 0) report_bad_index(a.status, kSiteScoredPage, page);
-      return -1;
-    }
-    return (((long long)page * a.Hkv + hb_ / pl.blocks) * a.page_size + (tok - col * a.page_size)) * D;
-  };
-  uint4 kx[2][NK], vx[D / 64][4];
-  auto load_k = [&](long long base) {
-    const T *p = static_cast<const T *>(a.k_cache) + (base < 0 ? 0 : base) + r * D + c * 8;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) kx[j][kk] = ld_stream(p + j * 8 * D + kk * 32);
-  };
-  auto load_v = [&](long long base) {
-    const T *p = static_cast<const T *>(a.v_cache) + (base < 0 ? 0 : base) + 2 * c * D + r * 8;
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) vx[i][j] = ld_stream(p + ((j & 1) + (j / 2) * 8) * D + i * 64);
-  };
-
-  float o[D / 8][ROWS / 4];
-  float m[RB], sum[RB];
-  auto clear = [&]() {
 #pragma unroll
     for (int i = 0; i < D / 8; ++i)
 #pragma unroll
       for (int j = 0; j < ROWS / 4; ++j) o[i][j] = 0.f;
 #pragma unroll
     for (int i = 0; i < RB; ++i) m[i] = -INFINITY, sum[i] = 0.f;
-  };
+  }
+  __device__ __forceinline__ void load_k(const ScoredArgs &a, long long base) {
+    const T *p = static_cast<const T *>(a.k_cache) + (base < 0 ? 0 : base) + r * D + c * 8;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) kx[j][kk] = ld_stream(p + j * 8 * D + kk * 32, policy);
+  }
+  __device__ __forceinline__ void load_v(const ScoredArgs &a, long long base) {
+    const T *p = static_cast<const T *>(a.v_cache) + (base < 0 ? 0 : base) + 2 * c * D + r * 8;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) vx[i][j] = ld_stream(p + ((j & 1) + (j / 2) * 8) * D + i * 64, policy);
+  }
 
-  long long base = tile_row(req, hb, tile);
-  load_k(base);
-  load_v(base);
-  enter_task();
-  clear();
-  int nt = tiles_of(n);
-  while (true) {
-    --left;
-    int n_req = req, n_hb = hb, n_tile = tile + 1, n_n = n;
-    const bool task_ends = n_tile == nt || left == 0;
-    long long next = -1;
-    if (left > 0) {
-      if (n_tile == nt) {
-        n_tile = 0;
-        if (++n_hb == HB) {
-          n_hb = 0;
-          do n_n = checked_len(a.kv_lens[++n_req], cap, nullptr, 0, false);
-          while (n_n == 0);  // more tiles follow, so a request with some does
-        }
-      }
-      next = tile_row(n_req, n_hb, n_tile);
-    }
+  // One tile, whose K and V are loaded or on their way: its logits go to
+  // s_out (row 0, the tile's first token; `pitch` between rows). With `more`,
+  // the tile at `next` is requested on the way.
+  __device__ __forceinline__ void step(const ScoredArgs &a, long long base, int tok, int n, float scale2, const QTile &q_sm,
+                                       float *s_out, int pitch, bool more, long long next) {
     float s[2][4];
 #pragma unroll
     for (int j = 0; j < 2; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk) {
-      const uint4 q0 = q_sm[warp][0][kk][lane];
-      const uint4 q1 = ROWS == 16 ? q_sm[warp][RB - 1][kk][lane] : make_uint4(0, 0, 0, 0);
+      const uint4 q0 = q_sm[0][kk][lane];
+      const uint4 q1 = ROWS == 16 ? q_sm[RB - 1][kk][lane] : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         mma16816<T>(s[j][0], s[j][1], s[j][2], s[j][3], q0.x, q1.x, q0.y, q1.y, kx[j][kk].x, kx[j][kk].y);
         mma16816<T>(s[j][0], s[j][1], s[j][2], s[j][3], q0.z, q1.z, q0.w, q1.w, kx[j][kk].z, kx[j][kk].w);
       }
     }
-    if (left > 0) load_k(next);
+    if (more) load_k(a, next);
     // tokens from `end` on are not there (behind the request's end, or their page is bad)
-    const int tok = tile * kTile;
     const int end = base < 0 ? tok : n;
     const bool whole = tok + kTile <= min(end, all_see);
     uint32_t pa[2][2] = {{0u, 0u}, {0u, 0u}};  // [row block][tile half]: P as the product's A operand
-    const int row0 = (hb % pl.blocks) * ROWS;
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
       float v[4] = {s[0][2 * i] * scale2, s[0][2 * i + 1] * scale2, s[1][2 * i] * scale2, s[1][2 * i + 1] * scale2};
@@ -425,8 +376,8 @@ __global__ void __launch_bounds__(kWarps * 32, kResident)
         for (int j = 0; j < 4; ++j)
           if (tok + (j / 2) * 8 + 2 * c + (j & 1) >= seen) v[j] = -INFINITY;
       }
-      if (row0 + r + 8 * i < pl.rows) {
-        float *dst = s_out + (size_t)(8 * i) * pl.lp + tok;
+      if (r + 8 * i < rows_here) {
+        float *dst = s_out + (size_t)(r + 8 * i) * pitch + 2 * c;
         *reinterpret_cast<float2 *>(dst) = make_float2(v[0], v[1]);
         *reinterpret_cast<float2 *>(dst + 8) = make_float2(v[2], v[3]);
       }
@@ -512,34 +463,130 @@ __global__ void __launch_bounds__(kWarps * 32, kResident)
         }
       }
     }
-    if (left > 0) load_v(next);
-    if (task_ends) {
-      const size_t part = (size_t)w_id + (uint32_t)req * HB + hb;
+    if (more) load_v(a, next);
+  }
+
+  // The partial result of the tiles since enter(): [rows][D] sums to o_out,
+  // (max, sum) to ml_out.
+  __device__ __forceinline__ void finish(float *o_out, float2 *ml_out) {
 #pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-        const int row = r + 8 * i;
-        if (row0 + row < pl.rows) {
-          float *dst = a.ws + pl.o_off + (part * ROWS + row) * D + 16 * c;
+    for (int i = 0; i < RB; ++i) {
+      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+      const int row = r + 8 * i;
+      if (row < rows_here) {
+        float *dst = o_out + row * D + 16 * c;
 #pragma unroll
-          for (int d = 0; d < D / 64; ++d)
+        for (int d = 0; d < D / 64; ++d)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-              const int x = d * 8 + e % 8, y = 2 * i + e / 8;
-              *reinterpret_cast<float4 *>(dst + d * 64 + e) = make_float4(o[x][y], o[x + 1][y], o[x + 2][y], o[x + 3][y]);
-            }
-          if (c == 0) reinterpret_cast<float2 *>(a.ws + pl.ml_off)[part * ROWS + row] = make_float2(m[i], sum[i]);
-        }
+          for (int e = 0; e < 16; e += 4) {
+            const int x = d * 8 + e % 8, y = 2 * i + e / 8;
+            *reinterpret_cast<float4 *>(dst + d * 64 + e) = make_float4(o[x][y], o[x + 1][y], o[x + 2][y], o[x + 3][y]);
+          }
+        if (c == 0) ml_out[row] = make_float2(m[i], sum[i]);
       }
-      if (left == 0) return;
-      req = n_req, hb = n_hb, n = n_n;
-      nt = tiles_of(n);
-      enter_task();
-      clear();
     }
-    tile = n_tile;
-    base = next;
+  }
+};
+
+// One warp: a run of the tile list.
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kWarps * 32, kResident)
+    scored_split_kernel(const ScoredArgs a, const ScoredPlan pl) {
+  __shared__ typename RowSoftmax<T, D, ROWS>::QTile q_sm[kWarps];
+  ptx::pdl_launch_dependents();
+  ptx::pdl_wait();
+  RowSoftmax<T, D, ROWS> x;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int cap = table_cap(a.max_len, a.bt_pages, a.page_size);
+  const int HB = a.Hkv * pl.blocks;
+  const uint32_t w_id = blockIdx.x * kWarps + warp;
+  auto tiles_of = [&](int n) { return (n + kTile - 1) / kTile; };
+
+  // this warp's run of the list (its length fits 31 bits)
+  uint32_t total = 0;
+  for (int i = lane; i < a.R; i += 32) total += tiles_of(checked_len(a.kv_lens[i], cap, a.status, kSiteScoredLen, w_id == 0));
+  total = __reduce_add_sync(0xffffffffu, total) * HB;
+  const uint32_t per = run_length(total, gridDim.x * kWarps);
+  if (w_id == 0) {  // for the join
+    uint32_t *meta = reinterpret_cast<uint32_t *>(a.ws + pl.meta_off);
+    uint32_t before = 0;
+    for (int i0 = 0; i0 < a.R; i0 += 32) {
+      const int len = i0 + lane < a.R ? checked_len(a.kv_lens[i0 + lane], cap, nullptr, 0, false) : 0;
+      const uint32_t own = tiles_of(len);
+      uint32_t inc = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (i0 + lane < a.R) meta[1 + 2 * (i0 + lane)] = len, meta[2 + 2 * (i0 + lane)] = before + inc - own;
+      before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) meta[0] = per;
+  }
+  if ((unsigned long long)w_id * per >= total) return;
+  const uint32_t u0 = w_id * per;
+  uint32_t left = min(per, total - u0);
+  int req = 0, hb = 0, tile = 0;
+  {
+    uint32_t before = 0;  // tiles (of one head) in front of request i0
+    for (int i0 = 0;; i0 += 32) {
+      const uint32_t own = i0 + lane < a.R ? tiles_of(checked_len(a.kv_lens[i0 + lane], cap, nullptr, 0, false)) : 0;
+      uint32_t inc = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, (before + inc) * HB > u0);
+      if (past != 0u) {
+        const int at = __ffs(past) - 1;
+        const uint32_t off = u0 - (before + __shfl_sync(0xffffffffu, inc - own, at)) * HB;
+        const uint32_t nt = __shfl_sync(0xffffffffu, own, at);
+        req = i0 + at;
+        hb = (int)(off / nt);
+        tile = (int)(off - (uint32_t)hb * nt);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+  }
+  int n = checked_len(a.kv_lens[req], cap, nullptr, 0, false);
+  const float scale2 = a.sm_scale * kLog2e;
+  long long base = tile_base(a, req, hb / pl.blocks, tile * kTile);
+  x.load_k(a, base);
+  x.load_v(a, base);
+  while (true) {  // a task
+    const int h = hb / pl.blocks, row0 = (hb - h * pl.blocks) * ROWS, nt = tiles_of(n);
+    x.enter(a, pl.rows, req, h, row0, n, q_sm[warp]);
+    float *s_out = a.ws + pl.s_off + (((size_t)req * a.Hkv + h) * pl.rows + row0) * pl.lp;
+    int n_req = req, n_hb = hb, n_n = n;
+    while (true) {  // a tile
+      --left;
+      const bool ends = tile + 1 == nt || left == 0;
+      int n_tile = tile + 1;
+      long long next = -1;
+      if (left > 0) {
+        if (ends) {
+          n_tile = 0;
+          if (++n_hb == HB) {
+            n_hb = 0;
+            do n_n = checked_len(a.kv_lens[++n_req], cap, nullptr, 0, false);
+            while (n_n == 0);  // more tiles follow, so a request with some does
+          }
+        }
+        next = tile_base(a, n_req, n_hb / pl.blocks, n_tile * kTile);
+      }
+      x.step(a, base, tile * kTile, n, scale2, q_sm[warp], s_out + tile * kTile, pl.lp, left > 0, next);
+      tile = n_tile;
+      base = next;
+      if (ends) break;
+    }
+    const size_t part = (size_t)w_id + (uint32_t)req * HB + hb;
+    x.finish(a.ws + pl.o_off + part * ROWS * D, reinterpret_cast<float2 *>(a.ws + pl.ml_off) + part * ROWS);
+    if (left == 0) return;
+    req = n_req, hb = n_hb, n = n_n;
   }
 }
 
@@ -547,15 +594,146 @@ __device__ __forceinline__ void red_add4(float *p, const float4 &v) {
   asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                : "memory");
 }
+// Adds the weights of tokens tok .. tok + 3 (those below `end`) to their scores.
+__device__ __forceinline__ void add_weights(const ScoredArgs &a, int req, int h, int tok, int end, const float4 &w) {
+  const int col = tok / a.page_size, page = a.block_table[(size_t)req * a.bt_stride + col];
+  if (page < 0 || page >= a.num_pages) return;  // reported where K was read
+  float *dst = a.scores + ((size_t)page * a.Hkv + h) * a.page_size + (tok - col * a.page_size);
+  if (tok + 4 <= end) {
+    red_add4(dst, w);
+  } else {
+    atomicAdd(dst, w.x);
+    if (tok + 1 < end) atomicAdd(dst + 1, w.y);
+    if (tok + 2 < end) atomicAdd(dst + 2, w.z);
+  }
+}
+__device__ __forceinline__ void add_weight(float4 &w, const float4 &s, float lse2) {
+  w.x += ex2_approx(s.x - lse2);
+  w.y += ex2_approx(s.y - lse2);
+  w.z += ex2_approx(s.z - lse2);
+  w.w += ex2_approx(s.w - lse2);
+}
 
-// Join. The first CTAs of a (request, KV head) join the outputs of two rows
-// each (four warps to a row, each a quarter of the partial results); the
-// others add the weights of pl.join tokens each: a thread has four tokens and
-// every groups-th row, whose logits it requests before the rows' lse is known.
-// All sums have a fixed order, and one request's pages get one addition per
-// token and head from a call.
+// The same in one kernel, for few and short contexts, where latency counts: a
+// cluster has a (request, KV head), its warps the tiles in turn (so that a
+// warp's first page does not depend on the length). The logits stay in shared
+// memory; the CTAs exchange (max, sum) and outputs through it, and each then
+// adds its own tokens' weights.
+constexpr int kCluster = 8;   // CTAs
+constexpr int kCWarps = 8;    // warps of each
+constexpr int kCTiles = 8;    // tiles of a warp at most (8192 tokens)
+
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kCWarps * 32) scored_cluster_kernel(const ScoredArgs a, int rows, int span) {
+  constexpr int NT = kCWarps * 32;
+  extern __shared__ __align__(16) float sm[];
+  __shared__ typename RowSoftmax<T, D, ROWS>::QTile q_sm[kCWarps];
+  __shared__ float2 ml_w[kCWarps][ROWS], ml_c[ROWS];
+  __shared__ float lse2[ROWS];                // +inf for a row that sees nothing
+  float *o_w = sm;                            // [kCWarps][ROWS][D]; the first [ROWS][D] then hold the CTA's
+  float *s_sm = sm + kCWarps * ROWS * D;      // [rows][span]
+  const int rank = (int)ptx::cluster_ctarank();
+  const int req = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int G = a.Hq / a.Hkv;
+  ptx::pdl_launch_dependents();
+  ptx::pdl_wait();
+  const int cap = table_cap(a.max_len, a.bt_pages, a.page_size);
+  int tile = rank + kCluster * warp;
+  const int page0 = tile * kTile < cap ? a.block_table[(size_t)req * a.bt_stride + tile * kTile / a.page_size] : -1;
+  const int n = checked_len(a.kv_lens[req], cap, a.status, kSiteScoredLen, h == 0 && rank == 0 && tid == 0);
+  const int nt = (n + kTile - 1) / kTile;
+  RowSoftmax<T, D, ROWS> x;
+  long long base = -1;
+  if (tile < nt) {
+    base = page_base(a, page0, h, tile * kTile);
+    x.load_k(a, base);
+    x.load_v(a, base);
+  }
+  x.enter(a, rows, req, h, 0, n, q_sm[warp]);
+  const float scale2 = a.sm_scale * kLog2e;
+  for (int at = warp * kTile; tile < nt; at += kCWarps * kTile) {
+    const int n_tile = tile + kCluster * kCWarps;
+    const long long next = n_tile < nt ? tile_base(a, req, h, n_tile * kTile) : -1;
+    x.step(a, base, tile * kTile, n, scale2, q_sm[warp], s_sm + at, span, n_tile < nt, next);
+    tile = n_tile;
+    base = next;
+  }
+  x.finish(o_w + warp * ROWS * D, ml_w[warp]);
+  __syncthreads();
+  // this CTA's sums, in warp order, relative to its own maximum
+  for (int i = tid; i < rows * D; i += NT) {
+    const int row = i / D;
+    float top = -INFINITY, tot = 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kCWarps; ++w) top = fmaxf(top, ml_w[w][row].x);
+#pragma unroll
+    for (int w = 0; w < kCWarps; ++w) {
+      const float f = scale_to(ml_w[w][row].x, top);
+      tot += ml_w[w][row].y * f;
+      v += o_w[w * ROWS * D + i] * f;
+    }
+    o_w[i] = v;
+    if (i % D == 0) ml_c[row] = make_float2(top, tot);
+  }
+  ptx::cluster_sync_all();
+  const uint32_t ml_addr = ptx::smem_u32(ml_c), o_addr = ptx::smem_u32(o_w);
+  auto peer2 = [&](uint32_t addr, int cta) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(ptx::mapa_shared(addr, cta)) : "memory");
+    return v;
+  };
+  {  // eight lanes to a row: a CTA's (max, sum) each
+    const int row = tid / kCluster, at = min(row, rows - 1);
+    const float2 mine = peer2(ml_addr + at * 8, tid % kCluster);
+    float top = mine.x;
+#pragma unroll
+    for (int o = kCluster / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float tot = mine.y * scale_to(mine.x, top);
+#pragma unroll
+    for (int o = kCluster / 2; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
+    const float v = top == -INFINITY && tot == 0.f ? -INFINITY : top + log2f(tot);  // NaN logits stay NaN
+    if (row < rows && tid % kCluster == 0) {
+      lse2[row] = v == -INFINITY ? INFINITY : v;
+      if (rank == 0 && a.lse != nullptr) {
+        const int qi = row / G;
+        a.lse[((size_t)req * a.Q + qi) * a.Hq + h * G + (row - qi * G)] = v * kLn2;
+      }
+    }
+  }
+  __syncthreads();
+  // outputs: two values a thread, spread over the cluster
+  for (int i = (rank * NT + tid) * 2; i < rows * D; i += kCluster * NT * 2) {
+    const int row = i / D, qi = row / G;
+    const float ref = lse2[row];
+    float2 m[kCluster], p[kCluster], v = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kCluster; ++k) m[k] = peer2(ml_addr + row * 8, k), p[k] = peer2(o_addr + i * 4, k);
+#pragma unroll
+    for (int k = 0; k < kCluster; ++k) {
+      const float f = ex2_approx(m[k].x - ref);
+      if (f != 0.f) v.x += p[k].x * f, v.y += p[k].y * f;
+    }
+    *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + (size_t)req * a.out_req + (size_t)qi * a.out_query +
+                                  (size_t)(h * G + row - qi * G) * D + i % D) = pack2<T>(v.x, v.y);
+  }
+  for (int q = tid; q < span / 4; q += NT) {  // four tokens of a tile that this CTA had
+    const int at = q * 4 / kTile, tok = ((at / kCWarps * kCWarps + at % kCWarps) * kCluster + rank) * kTile + q * 4 % kTile;
+    if (tok >= n) continue;
+    float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int row = 0; row < rows; ++row) add_weight(w, *reinterpret_cast<const float4 *>(s_sm + row * span + q * 4), lse2[row]);
+    add_weights(a, req, h, tok, n, w);
+  }
+  ptx::cluster_sync_all();  // the peers have read this CTA's shared memory
+}
+
+// Join. Of a (request, KV head)'s CTAs the first ones join the outputs
+// (pl.o_rows rows each, the warps shared evenly by them), the others add the
+// weights of pl.join tokens each: a thread has four tokens and every
+// groups-th row, whose logits it requests before the rows' lse is known. All
+// sums have a fixed order, and one request's pages get one addition per token
+// and head from a call.
 constexpr int kJoin = 256;
-constexpr int kJoinRows = 2;
+constexpr int kJoinWarps = kJoin / 32;
 
 // Partial results of a task: first index and count.
 struct Parts {
@@ -589,53 +767,26 @@ __device__ __forceinline__ float row_lse2(const float2 *ml, uint32_t count, int 
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoin) scored_join_kernel(const ScoredArgs a, const ScoredPlan pl, int o_ctas) {
+__global__ void __launch_bounds__(kJoin, 4) scored_join_kernel(const ScoredArgs a, const ScoredPlan pl, int o_ctas) {
   extern __shared__ __align__(16) float sm[];
-  __shared__ uint32_t red[2][kJoin / 32];
   ptx::pdl_launch_dependents();
   ptx::pdl_wait();
   const int req = blockIdx.z, h = blockIdx.y;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int cap = table_cap(a.max_len, a.bt_pages, a.page_size);
-  const int n = checked_len(a.kv_lens[req], cap, nullptr, 0, false);
-  const bool weigh = (int)blockIdx.x >= o_ctas;
-  const int t0 = ((int)blockIdx.x - o_ctas) * pl.join, t1 = min(n, t0 + pl.join);
-  if (weigh && t0 >= n) return;
-  const int G = a.Hq / a.Hkv, HB = a.Hkv * pl.blocks, nt = (n + kTile - 1) / kTile;
-
-  // this thread's first logits
-  constexpr int PRE = 4;
-  const int quads = min(pl.join / 4, kJoin), groups = kJoin / quads, grp = tid / quads, quad = tid % quads;
-  const float *s_in = a.ws + pl.s_off + ((size_t)req * a.Hkv + h) * pl.rows * pl.lp;
-  float4 pre[PRE];
-  if (weigh && t0 + quad * 4 < t1) {
-#pragma unroll
-    for (int j = 0; j < PRE; ++j)
-      if (grp + j * groups < pl.rows)
-        pre[j] = *reinterpret_cast<const float4 *>(s_in + (size_t)(grp + j * groups) * pl.lp + t0 + quad * 4);
-  }
-  uint32_t before = 0, total = 0;
-  for (int i = tid; i < a.R; i += kJoin) {
-    const uint32_t t = (uint32_t)(checked_len(a.kv_lens[i], cap, nullptr, 0, false) + kTile - 1) / kTile;
-    total += t;
-    if (i < req) before += t;
-  }
-  before = __reduce_add_sync(0xffffffffu, before);
-  total = __reduce_add_sync(0xffffffffu, total);
-  if (lane == 0) red[0][warp] = before, red[1][warp] = total;
-  __syncthreads();
-  before = total = 0;
-#pragma unroll
-  for (int w = 0; w < kJoin / 32; ++w) before += red[0][w], total += red[1][w];
-  const uint32_t per = run_length(total * HB, (uint32_t)(pl.grid * kWarps));
+  const uint32_t *meta = reinterpret_cast<const uint32_t *>(a.ws + pl.meta_off);
+  const int n = (int)meta[1 + 2 * req];
+  const uint32_t before = meta[2 + 2 * req], per = meta[0];
+  const int HB = a.Hkv * pl.blocks, nt = (n + kTile - 1) / kTile;
   const float2 *ml = reinterpret_cast<const float2 *>(a.ws + pl.ml_off);
 
-  if (!weigh) {
-    constexpr int SUB = kJoin / 32 / kJoinRows, V = D / 32;  // warps per row, values per lane
-    const int row = blockIdx.x * kJoinRows + warp / SUB, sub = warp % SUB;
+  if ((int)blockIdx.x < o_ctas) {
+    constexpr int V = D / 32;  // values per lane
+    const int sub = kJoinWarps / pl.o_rows, row = blockIdx.x * pl.o_rows + warp / sub, part = warp % sub;
+    if (sub == 1 && row >= pl.rows) return;
     float v[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = 0.f;
+    const int G = a.Hq / a.Hkv, qi = row / G;
     if (row < pl.rows) {
       const Parts pt = parts_of(before, per, nt, HB, req, h * pl.blocks + row / pl.block);
       const float2 *mr = ml + (size_t)pt.first * pl.block + row % pl.block;
@@ -643,7 +794,7 @@ __global__ void __launch_bounds__(kJoin) scored_join_kernel(const ScoredArgs a, 
       const float ref = lse2 == -INFINITY ? INFINITY : lse2;
       const float *src = a.ws + pl.o_off + ((size_t)pt.first * pl.block + row % pl.block) * D + lane * V;
 #pragma unroll 4
-      for (uint32_t k = sub; k < pt.count; k += SUB) {
+      for (uint32_t k = part; k < pt.count; k += sub) {
         const float f = ex2_approx(mr[(size_t)k * pl.block].x - ref);
         float p[V];
         if constexpr (V == 4)
@@ -653,60 +804,72 @@ __global__ void __launch_bounds__(kJoin) scored_join_kernel(const ScoredArgs a, 
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] += f != 0.f ? p[e] * f : 0.f;
       }
-      if (sub == 0 && lane == 0 && a.lse != nullptr) {
-        const int qi = row / G;
+      if (part == 0 && lane == 0 && a.lse != nullptr)
         a.lse[((size_t)req * a.Q + qi) * a.Hq + h * G + (row - qi * G)] = lse2 * kLn2;
-      }
     }
+    if (sub > 1) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) sm[warp * D + lane * V + e] = v[e];
-    __syncthreads();
-    if (row < pl.rows && sub == 0) {
-      const int qi = row / G;
-      T *dst = static_cast<T *>(a.out) + (size_t)req * a.out_req + (size_t)qi * a.out_query + (size_t)(h * G + row - qi * G) * D;
+      for (int e = 0; e < V; ++e) sm[warp * D + lane * V + e] = v[e];
+      __syncthreads();
+      if (row >= pl.rows || part != 0) return;
+      for (int w = 1; w < sub; ++w)
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-#pragma unroll
-        for (int w = 1; w < SUB; ++w) v[e] += sm[(warp + w) * D + lane * V + e];
-        dst[lane * V + e] = narrow<T>(v[e]);
-      }
+        for (int e = 0; e < V; ++e) v[e] += sm[(warp + w) * D + lane * V + e];
     }
+    T *dst = static_cast<T *>(a.out) + (size_t)req * a.out_req + (size_t)qi * a.out_query + (size_t)(h * G + row - qi * G) * D + lane * V;
+    if constexpr (V == 4)
+      *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    else
+      *reinterpret_cast<uint32_t *>(dst) = pack2<T>(v[0], v[1]);
     return;
   }
 
+  const int t0 = ((int)blockIdx.x - o_ctas) * pl.join, t1 = min(n, t0 + pl.join);
+  if (t0 >= n) return;
+  constexpr int PRE = 4;
+  const int quads = min(pl.join / 4, kJoin), groups = kJoin / quads, grp = tid / quads, quad = tid % quads;
+  const float *s_in = a.ws + pl.s_off + ((size_t)req * a.Hkv + h) * pl.rows * pl.lp;
+  float4 pre[PRE];
+  auto prefetch = [&](int tok) {
+    if (tok < t1) {
+#pragma unroll
+      for (int j = 0; j < PRE; ++j)
+        if (grp + j * groups < pl.rows)
+          pre[j] = *reinterpret_cast<const float4 *>(s_in + (size_t)(grp + j * groups) * pl.lp + tok);
+    }
+  };
+  prefetch(t0 + quad * 4);
   float4 *part_w = reinterpret_cast<float4 *>(sm);  // [kJoin]
   float *lse2 = sm + 4 * kJoin;                     // [rows]: +inf for a row that sees nothing
-  constexpr int LR = 8;                             // lanes per row
-  for (int row = tid / LR; row - tid / LR < pl.rows; row += kJoin / LR) {
-    const bool in = row < pl.rows;
-    const Parts pt = parts_of(before, per, nt, HB, req, h * pl.blocks + (in ? row : 0) / pl.block);
-    const float v = row_lse2<LR>(ml + (size_t)pt.first * pl.block + (in ? row : 0) % pl.block, pt.count, pl.block);
-    if (in && tid % LR == 0) lse2[row] = v == -INFINITY ? INFINITY : v;
+  auto put_lse = [&](int row, float v) { lse2[row] = v == -INFINITY ? INFINITY : v; };
+  if (pl.rows <= kJoinWarps) {
+    if (warp < pl.rows) {
+      const Parts pt = parts_of(before, per, nt, HB, req, h);
+      const float v = row_lse2<32>(ml + (size_t)pt.first * pl.block + warp, pt.count, pl.block);
+      if (lane == 0) put_lse(warp, v);
+    }
+  } else {
+    constexpr int LR = 8;  // lanes per row
+    for (int row = tid / LR; row - tid / LR < pl.rows; row += kJoin / LR) {
+      const int at = min(row, pl.rows - 1);
+      const Parts pt = parts_of(before, per, nt, HB, req, h * pl.blocks + at / pl.block);
+      const float v = row_lse2<LR>(ml + (size_t)pt.first * pl.block + at % pl.block, pt.count, pl.block);
+      if (row < pl.rows && tid % LR == 0) put_lse(row, v);
+    }
   }
   __syncthreads();
   for (int tq = t0; tq < t1; tq += quads * 4) {
     const int tok = tq + quad * 4;
     float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](const float4 &s, float ref) {
-      w.x += ex2_approx(s.x - ref);
-      w.y += ex2_approx(s.y - ref);
-      w.z += ex2_approx(s.z - ref);
-      w.w += ex2_approx(s.w - ref);
-    };
     if (tok < t1) {
 #pragma unroll
       for (int j = 0; j < PRE; ++j)
-        if (grp + j * groups < pl.rows) add(pre[j], lse2[grp + j * groups]);
+        if (grp + j * groups < pl.rows) add_weight(w, pre[j], lse2[grp + j * groups]);
 #pragma unroll 4
       for (int row = grp + PRE * groups; row < pl.rows; row += groups)
-        add(*reinterpret_cast<const float4 *>(s_in + (size_t)row * pl.lp + tok), lse2[row]);
+        add_weight(w, *reinterpret_cast<const float4 *>(s_in + (size_t)row * pl.lp + tok), lse2[row]);
     }
-    if (tok + quads * 4 < t1) {
-#pragma unroll
-      for (int j = 0; j < PRE; ++j)
-        if (grp + j * groups < pl.rows)
-          pre[j] = *reinterpret_cast<const float4 *>(s_in + (size_t)(grp + j * groups) * pl.lp + tok + quads * 4);
-    }
+    prefetch(tok + quads * 4);
     if (groups > 1) {
       part_w[tid] = w;
       __syncthreads();
@@ -717,17 +880,7 @@ __global__ void __launch_bounds__(kJoin) scored_join_kernel(const ScoredArgs a, 
         }
       __syncthreads();
     }
-    if (grp != 0 || tok >= t1) continue;
-    const int col = tok / a.page_size, page = a.block_table[(size_t)req * a.bt_stride + col];
-    if (page < 0 || page >= a.num_pages) continue;  // reported by the split kernel
-    float *dst = a.scores + ((size_t)page * a.Hkv + h) * a.page_size + (tok - col * a.page_size);
-    if (tok + 4 <= t1) {
-      red_add4(dst, w);
-    } else {
-      atomicAdd(dst, w.x);
-      if (tok + 1 < t1) atomicAdd(dst + 1, w.y);
-      if (tok + 2 < t1) atomicAdd(dst + 2, w.z);
-    }
+    if (grp == 0 && tok < t1) add_weights(a, req, h, tok, t1, w);
   }
 }
 
@@ -738,200 +891,356 @@ __global__ void __launch_bounds__(kJoin) scored_join_kernel(const ScoredArgs a, 
 // NaN and -inf lowest. Kept tokens in slots >= budget then take the slots
 // < budget of evicted ones, the i-th the i-th: sources and destinations are
 // disjoint, so the moves need no order and only they touch K and V.
-constexpr int kSelThreads = 1024;
-constexpr int kSelBins = 4096;
+constexpr int kBins = 2048;          // of a selection digit: 11, 11 and 10 bits
+constexpr int kFew = 256;            // keys that one warp finishes the selection of, eight a lane
+constexpr int kWindow = 1024;        // moves a CTA lists at a time
+constexpr int kKeySmem = 40 * 1024;  // slots whose keys fit shared memory; longer contexts keep them in the workspace
+constexpr uint32_t kNoRow = 0xffffffffu;
 
-__device__ __forceinline__ uint32_t evict_key(float score, int pos, int last, int recent, int sink) {
-  if ((long long)pos > (long long)last - recent || pos < sink) return 0xffffffffu;
-  if (!(score == score)) score = -INFINITY;
-  const uint32_t u = __float_as_uint(score + 0.f);  // -0 counts as 0
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+// `after`: the position behind which tokens are recent
+__device__ __forceinline__ uint32_t evict_key(float score, int pos, int after, int sink) {
+  const uint32_t u = __float_as_uint((score == score ? score : -INFINITY) + 0.f);  // -0 counts as 0
+  const uint32_t k = u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+  return pos > after || pos < sink ? 0xffffffffu : k;
 }
 
-// Radix selection of the budget-th largest key in digits of 12, 10 and 10
-// bits, then two ordered sweeps (each warp owns a run of slots, so ranks come
-// from ballots and one prefix over the warps) that list the movers and holes.
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const KvEvictArgs a, int list_cap,
-                                                                   int32_t *key_ws) {
-  extern __shared__ uint32_t keys_sm[];  // [max_len] unless the keys are in the workspace
-  __shared__ uint32_t hist[kSelBins];
-  __shared__ uint32_t wsum[32], s_bin, s_above;
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) >= o) v += u;
+  }
+  return v;
+}
+
+// Words a CTA needs for n slots: a key each, and a flag word and its prefix
+// for every 32; a multiple of 16 bytes, so that every CTA's keys start on one.
+__host__ __device__ __forceinline__ size_t evict_words(int n) { return ((size_t)((n + 31) / 32) * (32 + 2) + 3) / 4 * 4; }
+
+// A cluster has a (request, KV head). Every CTA of it finds the budget-th
+// largest key by radix selection over all the keys (8 bytes a token to read;
+// doing it once more per CTA costs less than exchanging histograms), and once
+// all of them have read the scores, each moves its share of the tokens.
+//
+// The last key kept and, among its equals, the last slot kept decide each
+// slot. A flag marks the slots below the budget that lose their token and the
+// slots behind it that keep theirs; as many of the one as of the other, so one
+// prefix sum over the flags ranks both.
+template <int D>
+__global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32_t *ws, int vec, int page_shift) {
+  extern __shared__ __align__(16) uint32_t dyn[];  // evict_words(max_len) unless they are in the workspace
+  __shared__ __align__(16) uint32_t hist[kBins];
+  __shared__ uint32_t tot[32], s_bin, s_above, s_count, s_found, s_key;
+  __shared__ int s_slot;
+  __shared__ __align__(16) uint32_t from[kWindow], to[kWindow];  // slots, then cache rows, of the moves; keys and slots before
+  const int tid = threadIdx.x, NT = blockDim.x, NW = NT / 32, warp = tid / 32, lane = tid % 32;
+  const int rank = (int)ptx::cluster_ctarank(), C = (int)ptx::cluster_nctarank();
+  const int req = blockIdx.z, h = blockIdx.y;
+  for (int i = tid; i < kBins; i += NT) hist[i] = 0;
+  if (tid == 0) s_found = 0;
   ptx::pdl_launch_dependents();
   ptx::pdl_wait();
-  const int h = blockIdx.x, req = blockIdx.y;
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int cap = min(a.max_len, (int)min((long long)a.bt_pages * a.page_size, 0x7fffffffll));
-  const int n = checked_len(a.kv_lens[req], cap, a.status, kSiteEvictLen, h == 0 && tid == 0);
+  const int cap = table_cap(a.max_len, a.bt_pages, a.page_size);
+  const int n = checked_len(a.kv_lens[req], cap, a.status, kSiteEvictLen, h == 0 && rank == 0 && tid == 0);
   const int b = a.budget;
-  if (h == 0 && tid == 0) a.new_lens[req] = min(n, b);
-  const size_t head = (size_t)req * a.Hkv + h;
-  int32_t *count = a.ws + head;
-  if (n <= b) {
-    if (tid == 0 && a.ws != nullptr) *count = 0;
-    return;
-  }
-  uint32_t *keys = key_ws == nullptr ? keys_sm : reinterpret_cast<uint32_t *>(key_ws) + head * (size_t)a.max_len;
+  if (h == 0 && rank == 0 && tid == 0) a.new_lens[req] = min(n, b);
+  if (n <= b) return;  // the whole cluster
   const int32_t *bt = a.block_table + (size_t)req * a.bt_stride;
-  const int last = a.last_pos[req];
-  for (int j = tid; j < n; j += kSelThreads) {
-    const int col = j / a.page_size, page = bt[col];
-    uint32_t k = 0u;
-    if (page < 0 || page >= a.num_pages) {
-      report_bad_index(a.status, kSiteEvictPage, page);
-    } else {
-      const size_t row = ((size_t)page * a.Hkv + h) * a.page_size + (j - col * a.page_size);
-      k = evict_key(a.scores[row], a.positions[row], last, a.recent, a.sink);
+  const int after = (int)max((long long)a.last_pos[req] - a.recent, -0x80000000ll);
+  uint32_t *keys = ws == nullptr ? dyn : ws + (((size_t)req * a.Hkv + h) * C + rank) * evict_words(a.max_len);
+  const int nw = (n + 31) / 32;
+  uint32_t *flags = keys + (size_t)nw * 32, *before = flags + nw;
+  // the row of a slot in the cache and in scores / positions, kNoRow for a bad page
+  auto row_of = [&](int j) {
+    const int col = page_shift >= 0 ? j >> page_shift : j / a.page_size, page = bt[col];
+    return page < 0 || page >= a.num_pages ? kNoRow : ((uint32_t)page * a.Hkv + h) * a.page_size + (j - col * a.page_size);
+  };
+  auto tell_bad = [&](int j) { report_bad_index(a.status, kSiteEvictPage, bt[j / a.page_size]); };
+  __syncthreads();
+  // the keys, and the histogram of their first digit. A page outside the
+  // cache is reported; its tokens have the lowest key.
+  if (vec) {  // four slots of one page at a time, UL such groups of a thread in flight
+    constexpr int UL = 3;
+    for (int j0 = tid * 4; j0 < n; j0 += NT * 4 * UL) {
+      uint32_t row[UL];
+      float4 s[UL];
+      int4 p[UL];
+#pragma unroll
+      for (int u = 0; u < UL; ++u) row[u] = j0 + u * NT * 4 < n ? row_of(j0 + u * NT * 4) : kNoRow;
+#pragma unroll
+      for (int u = 0; u < UL; ++u) {
+        const uint32_t at = row[u] == kNoRow ? 0u : row[u];
+        s[u] = *reinterpret_cast<const float4 *>(a.scores + at);
+        p[u] = *reinterpret_cast<const int4 *>(a.positions + at);
+      }
+#pragma unroll
+      for (int u = 0; u < UL; ++u) {
+        const int j = j0 + u * NT * 4;
+        if (j >= n) break;
+        uint4 k = make_uint4(evict_key(s[u].x, p[u].x, after, a.sink), evict_key(s[u].y, p[u].y, after, a.sink),
+                             evict_key(s[u].z, p[u].z, after, a.sink), evict_key(s[u].w, p[u].w, after, a.sink));
+        if (row[u] == kNoRow) {
+          k = make_uint4(0, 0, 0, 0);
+          tell_bad(j);
+        }
+        *reinterpret_cast<uint4 *>(keys + j) = k;
+        atomicAdd(&hist[k.x >> 21], 1u);
+        if (j + 1 < n) atomicAdd(&hist[k.y >> 21], 1u);
+        if (j + 2 < n) atomicAdd(&hist[k.z >> 21], 1u);
+        if (j + 3 < n) atomicAdd(&hist[k.w >> 21], 1u);
+      }
     }
-    keys[j] = k;
+  } else {
+    for (int j = tid; j < n; j += NT) {
+      const uint32_t row = row_of(j);
+      uint32_t k = 0u;
+      if (row == kNoRow)
+        tell_bad(j);
+      else
+        k = evict_key(a.scores[row], a.positions[row], after, a.sink);
+      keys[j] = k;
+      atomicAdd(&hist[k >> 21], 1u);
+    }
   }
+
   uint32_t prefix = 0, mask = 0;
-  uint32_t need = (uint32_t)b;  // keys still to keep among those that match the prefix
+  uint32_t need = (uint32_t)b;          // keys still to keep among those that match the prefix
+  int last_slot = 0x7fffffff;           // of the keys that match in the end, those up to this slot stay
+#pragma unroll 1
   for (int digit = 0; digit < 3; ++digit) {
-    const int bits = digit == 0 ? 12 : 10, shift = digit == 0 ? 20 : (digit == 1 ? 10 : 0);
-    const int bins = 1 << bits;
-    for (int i = tid; i < bins; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    for (int j = tid; j < n; j += kSelThreads) {
-      const uint32_t k = keys[j];
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
-    }
-    __syncthreads();
-    // bins from the top: thread t owns bins/1024 of them
-    const int per = bins / kSelThreads;
-    uint32_t own = 0;
-    for (int i = 0; i < per; ++i) own += hist[bins - 1 - (tid * per + i)];
-    uint32_t inc = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    if (lane == 31) wsum[warp] = inc;
-    __syncthreads();
-    if (warp == 0) {
-      uint32_t v = wsum[lane];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
+    const int shift = digit == 0 ? 21 : (digit == 1 ? 10 : 0);
+    const uint32_t top = digit == 2 ? 1023u : 2047u;
+    if (digit > 0) {
+      for (int j = tid; j < n; j += NT) {
+        const uint32_t k = keys[j];
+        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & top], 1u);
       }
-      wsum[lane] = v;
     }
     __syncthreads();
-    uint32_t above = inc - own + (warp > 0 ? wsum[warp - 1] : 0u);
-    for (int i = 0; i < per; ++i) {
-      const int bin = bins - 1 - (tid * per + i);
-      const uint32_t hv = hist[bin];
-      if (above < need && above + hv >= need) {
-        s_bin = (uint32_t)bin;
-        s_above = above;
+    // bins from the top, 2048 / NT of them a thread, cleared on the way for the next digit
+    uint32_t own[8], sum = 0;
+    const int per = kBins / NT;  // 8, 4 or 2
+    const int hi = kBins - 1 - tid * per;
+    if (per == 8) {
+      uint4 *q = reinterpret_cast<uint4 *>(hist + hi - 7);
+      const uint4 lo4 = q[0], hi4 = q[1];
+      q[0] = q[1] = make_uint4(0, 0, 0, 0);
+      own[0] = hi4.w, own[1] = hi4.z, own[2] = hi4.y, own[3] = hi4.x;
+      own[4] = lo4.w, own[5] = lo4.z, own[6] = lo4.y, own[7] = lo4.x;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) own[i] = i < per ? hist[hi - i] : 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < per) hist[hi - i] = 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += own[i];
+    const uint32_t inc = warp_scan(sum);
+    if (lane == 31) tot[warp] = inc;
+    __syncthreads();
+    const uint32_t front = warp_scan(lane < NW ? tot[lane] : 0u);
+    uint32_t above = inc - sum + (warp > 0 ? __shfl_sync(0xffffffffu, front, warp - 1) : 0u);
+    if (above < need && above + sum >= need) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (above < need && above + own[i] >= need) {
+          s_bin = (uint32_t)(hi - i);
+          s_above = above;
+          s_count = own[i];
+        }
+        above += own[i];
       }
-      above += hv;
     }
     __syncthreads();
     prefix |= s_bin << shift;
-    mask |= (uint32_t)(bins - 1) << shift;
+    mask |= top << shift;
     need -= s_above;
+    const uint32_t match = s_count;
+    if (match == need) break;  // all keys that match the digits so far stay: the other digits decide nothing
+    if (match <= kFew) {
+      // few keys match: one warp finishes, bit by bit, with the slots of the listed keys for ties
+      for (int j = tid; j < n; j += NT) {
+        const uint32_t k = keys[j];
+        if ((k & mask) == prefix) {
+          const uint32_t i = atomicAdd(&s_found, 1u);
+          from[i] = k;
+          to[i] = (uint32_t)j;
+        }
+      }
+      __syncthreads();
+      if (warp == 0) {
+        uint32_t k[kFew / 32];
+        int slot[kFew / 32];
+#pragma unroll
+        for (int i = 0; i < kFew / 32; ++i) {
+          const uint32_t at = i * 32 + lane;
+          k[i] = at < match ? from[at] : 0u;  // below any key that matches, or among its equals the last
+          slot[i] = at < match ? (int)to[at] : 0x7fffffff;
+        }
+        uint32_t key = prefix, equal = 0, more = 0;  // the largest key with `need` keys not below it
+        for (uint32_t bit = (1u << shift) >> 1; bit != 0; bit >>= 1) {
+          uint32_t c = 0;
+#pragma unroll
+          for (int i = 0; i < kFew / 32; ++i) c += slot[i] != 0x7fffffff && k[i] >= (key | bit);
+          if (__reduce_add_sync(0xffffffffu, c) >= need) key |= bit;
+        }
+#pragma unroll
+        for (int i = 0; i < kFew / 32; ++i) {
+          more += slot[i] != 0x7fffffff && k[i] > key;
+          equal += slot[i] != 0x7fffffff && k[i] == key;
+        }
+        more = __reduce_add_sync(0xffffffffu, more);
+        equal = __reduce_add_sync(0xffffffffu, equal);
+        int upto = 0x7fffffff;
+        if (more + equal > need) {  // of the equal ones, the lowest slots: the smallest bound with enough up to it
+          upto = 0;
+          for (int bit = 1 << (31 - __clz(n)); bit != 0; bit >>= 1) {
+            uint32_t c = 0;
+#pragma unroll
+            for (int i = 0; i < kFew / 32; ++i) c += k[i] == key && slot[i] < (upto | bit);
+            if (__reduce_add_sync(0xffffffffu, c) < need - more) upto |= bit;
+          }
+        }
+        if (lane == 0) s_key = key, s_slot = upto;
+      }
+      __syncthreads();
+      prefix = s_key;
+      mask = 0xffffffffu;
+      last_slot = s_slot;
+      break;
+    }
+    if (digit == 2) last_slot = -1;  // many equal keys: found by the prefix sum below
+  }
+
+  // Sets flags[w] to the slots j of word w for which f(j, key) holds and
+  // before[w] to the number of such slots in front of it; returns their total.
+  auto flag = [&](auto f) {
+#pragma unroll 4
+    for (int w = warp; w < nw; w += NW) {
+      const int j = w * 32 + lane;
+      const uint32_t word = __ballot_sync(0xffffffffu, j < n && f(j, j < n ? keys[j] & mask : 0u));
+      if (lane == 0) flags[w] = word;
+    }
+    __syncthreads();
+    uint32_t carry = 0;
+    for (int w0 = 0; w0 < nw; w0 += NT) {
+      const uint32_t c = w0 + tid < nw ? __popc(flags[w0 + tid]) : 0;
+      const uint32_t inc = warp_scan(c);
+      if (lane == 31) tot[warp] = inc;
+      __syncthreads();
+      const uint32_t front = warp_scan(lane < NW ? tot[lane] : 0u);
+      const uint32_t warps_ahead = __shfl_sync(0xffffffffu, front, max(warp - 1, 0));
+      if (w0 + tid < nw) before[w0 + tid] = carry + inc - c + (warp > 0 ? warps_ahead : 0u);
+      carry += __shfl_sync(0xffffffffu, front, 31);
+      __syncthreads();
+    }
+    return carry;
+  };
+  if (last_slot < 0) {
+    flag([&](int, uint32_t k) { return k == prefix; });
+    for (int w = tid; w < nw; w += NT) {  // the word with the need-th of them
+      const uint32_t f = flags[w], at = before[w];
+      if (at < need && at + __popc(f) >= need) s_slot = w * 32 + (int)__fns(f, 0, (int)(need - at));
+    }
+    __syncthreads();
+    last_slot = s_slot;
     __syncthreads();
   }
-  // keys > prefix stay, and the first `need` that equal it
-  const int seg = ((n + 31) / 32 + 31) / 32 * 32;  // slots per warp
-  const int w0 = warp * seg, w1 = min(n, w0 + seg);
-  uint32_t eq = 0;
-  for (int j = w0 + lane; j - lane < w1; j += 32)
-    eq += __popc(__ballot_sync(0xffffffffu, j < w1 && keys[j] == prefix));
-  if (lane == 0) wsum[warp] = eq;
-  __syncthreads();
-  uint32_t eq_base = 0;
-  for (int w = 0; w < warp; ++w) eq_base += wsum[w];
-  __syncthreads();
-  int32_t *movers = a.ws + (size_t)a.R * a.Hkv + head * 2 * (size_t)list_cap, *holes = movers + list_cap;
-  uint32_t base_h = 0, base_m = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    uint32_t eq_at = eq_base, nh = base_h, nm = base_m;
-    for (int j = w0 + lane; j - lane < w1; j += 32) {
-      const bool in = j < w1;
-      const uint32_t k = in ? keys[j] : 0u;
-      const uint32_t lower = (1u << lane) - 1u;
-      const uint32_t beq = __ballot_sync(0xffffffffu, in && k == prefix);
-      const bool keep = in && (k > prefix || (k == prefix && eq_at + __popc(beq & lower) < need));
-      eq_at += __popc(beq);
-      const bool hole = in && !keep && j < b, mover = keep && j >= b;
-      const uint32_t bh = __ballot_sync(0xffffffffu, hole), bm = __ballot_sync(0xffffffffu, mover);
-      if (pass == 1) {
-        if (hole) holes[nh + __popc(bh & lower)] = j;
-        if (mover) movers[nm + __popc(bm & lower)] = j;
-      }
-      nh += __popc(bh);
-      nm += __popc(bm);
-    }
-    if (pass == 0) {
-      if (lane == 0) hist[warp] = nh, hist[32 + warp] = nm;
-      __syncthreads();
-      uint32_t total = 0;
-      for (int w = 0; w < 32; ++w) {
-        if (w < warp) base_h += hist[w], base_m += hist[32 + w];
-        total += hist[32 + w];
-      }
-      if (tid == 0) *count = (int)total;
-      __syncthreads();
-    }
-  }
-}
+  const int moves = (int)(flag([&](int j, uint32_t k) {
+                            const bool keep = k > prefix || (k == prefix && j <= last_slot);
+                            return keep == (j >= b);
+                          }) / 2);
+  if (C > 1) ptx::cluster_sync_all();  // every CTA has read the scores: they may change
 
-// A warp moves a token's K and V rows (and its weight and position): the
-// list entry's two rows are found once per 32 entries, one per lane.
-template <int D>
-__global__ void __launch_bounds__(256) evict_move_kernel(const KvEvictArgs a, int list_cap) {
-  constexpr int LPR = D * 2 / 16;         // lanes per row
-  constexpr int TPW = 32 / (2 * LPR);     // tokens a warp moves at once (K and V rows)
-  ptx::pdl_launch_dependents();
-  ptx::pdl_wait();
-  const int h = blockIdx.y, req = blockIdx.z;
-  const size_t head = (size_t)req * a.Hkv + h;
-  const int m = a.ws[head];
-  const int32_t *movers = a.ws + (size_t)a.R * a.Hkv + head * 2 * (size_t)list_cap, *holes = movers + list_cap;
-  const int32_t *bt = a.block_table + (size_t)req * a.bt_stride;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  for (int i0 = (blockIdx.x * 8 + warp) * 32; i0 < m; i0 += gridDim.x * 8 * 32) {
-    long long src = -1, dst = -1;
-    if (i0 + lane < m) {
-      const int js = movers[i0 + lane], jd = holes[i0 + lane];
-      const int cs = js / a.page_size, cd = jd / a.page_size;
-      const int ps = bt[cs], pd = bt[cd];
-      if (ps >= 0 && ps < a.num_pages && pd >= 0 && pd < a.num_pages) {  // bad pages: reported by the selection
-        src = ((long long)ps * a.Hkv + h) * a.page_size + (js - cs * a.page_size);
-        dst = ((long long)pd * a.Hkv + h) * a.page_size + (jd - cd * a.page_size);
+  constexpr int LPR = D * 2 / 16;      // lanes per row
+  constexpr int TPW = 32 / (2 * LPR);  // tokens a warp moves at once (K and V rows)
+  constexpr int U = 4;
+  const int sub = lane / (2 * LPR), which = (lane / LPR) & 1, at = lane % LPR;
+  uint4 *cache = static_cast<uint4 *>(which ? a.v_cache : a.k_cache);
+  // the CTA's share of the ranks, kWindow at a time
+  const int share = (moves + C - 1) / C, r0 = min(moves, rank * share), r1 = min(moves, r0 + share);
+  for (int q0 = r0; q0 < r1; q0 += kWindow) {
+    const int cnt = min(r1 - q0, kWindow);
+    for (int w = warp; w < nw; w += NW) {
+      const uint32_t word = flags[w];
+      if (word >> lane & 1u) {
+        const int j = w * 32 + lane;
+        int i = (int)(before[w] + __popc(word & ((1u << lane) - 1u))) - q0;
+        uint32_t *list = to;
+        if (j >= b) i -= moves, list = from;
+        if (i >= 0 && i < cnt) list[i] = (uint32_t)j;
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < cnt; i += NT) {  // slots to rows, and the tracking entries
+      const uint32_t src = row_of((int)from[i]);
+      uint32_t dst = row_of((int)to[i]);
+      if (src == kNoRow) dst = kNoRow;  // a bad page, reported above
+      if (dst != kNoRow) {
         a.scores[dst] = a.scores[src];
         a.positions[dst] = a.positions[src];
       }
+      from[i] = src;
+      to[i] = dst;
     }
-    const int sub = lane / (2 * LPR), which = (lane / LPR) & 1, at = lane % LPR;
-    const uint4 *in = static_cast<const uint4 *>(which ? a.v_cache : a.k_cache);
-    uint4 *out = static_cast<uint4 *>(which ? a.v_cache : a.k_cache);
-    const int cnt = min(32, m - i0);
-    for (int i = 0; i < cnt; i += 4 * TPW) {
-      uint4 v[4];
-      long long to[4];
+    __syncthreads();
+    for (int i = warp * TPW + sub; i - sub < cnt; i += NW * TPW * U) {
+      uint4 v[U];
+      uint32_t out[U];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int e = i + u * TPW + sub;
-        const long long s = __shfl_sync(0xffffffffu, src, e & 31);
-        to[u] = __shfl_sync(0xffffffffu, dst, e & 31);
-        if (e >= cnt) to[u] = -1;
-        if (to[u] >= 0) v[u] = in[s * LPR + at];
+      for (int u = 0; u < U; ++u) {
+        const int e = i + u * NW * TPW;
+        out[u] = e < cnt ? to[e] : kNoRow;
+        if (out[u] != kNoRow) v[u] = cache[(size_t)from[e] * LPR + at];
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (to[u] >= 0) out[to[u] * LPR + at] = v[u];
+      for (int u = 0; u < U; ++u)
+        if (out[u] != kNoRow) cache[(size_t)out[u] * LPR + at] = v[u];
     }
+    __syncthreads();
   }
 }
 
-constexpr int kKeySmem = 40 * 1024;  // keys kept in shared memory (160 KB); longer contexts keep them in the workspace
+struct EvictPlan {
+  int threads, cluster;
+};
+inline EvictPlan evict_plan(int R, int Hkv, int max_len, int budget, int num_sms) {
+  EvictPlan p;
+  const long long heads = (long long)R * Hkv;
+  // about eight keys a thread (512 heads of 2112 slots: 20 us with 256 threads, 27 with 512; 128 heads of 8192: 53 us
+  // with 1024, 61 with 512)
+  p.threads = 256;
+  while (p.threads < 1024 && p.threads * 9 < max_len) p.threads *= 2;
+  // more CTAs per head while there are many tokens to move and SMs for them (one head of 30001 slots, 6227 moves:
+  // 97 us with one CTA, 29 with eight; where the heads fill the SMs a second CTA only selects once more)
+  const int list = budget < max_len - budget ? budget : max_len - budget;
+  p.cluster = 1;
+  while (p.cluster < 8 && list > 128 * p.cluster && heads * p.cluster * 2 * p.threads <= 1024ll * num_sms) p.cluster *= 2;
+  return p;
+}
 
 }  // namespace kvb
 
+// Launch with clusters along x, and programmatic stream serialization as launch_pdl.
+template <typename... KArgs, typename... Args>
+static int launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, int cluster, size_t smem, cudaStream_t st,
+                          Args &&...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...) == cudaSuccess ? 0 : -4;
+}
 static inline int launched() { return cudaPeekAtLastError() == cudaSuccess ? 0 : -4; }
 static inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -956,23 +1265,53 @@ extern "C" int sched_qk_norm_rope_kv_append(const QkNormArgs *args, cudaStream_t
   return launched();
 }
 
-extern "C" long long sched_attn_scored_ws_floats(int R, int Q, int Hq, int Hkv, int D, int max_len, int num_sms) {
-  if (R <= 0 || Q <= 0 || Hkv <= 0 || Hq < Hkv || max_len <= 0) return 0;
-  return kvb::scored_plan(R, Q, Hq, Hkv, D, max_len, num_sms).total;
-}
 
 namespace kvb {
+// The one-kernel form, for a few tiles a warp and clusters that are all
+// resident at once: one CTA to an SM with heads of 128 (by its registers), two
+// with 64, and of the SMs about three quarters, since a cluster lies within a
+// GPC (14 clusters of one-to-an-SM CTAs fit, 16 do not). One request of 700
+// tokens, 8 heads of 128: 6.3 us against 9.3 with two kernels, of 8000: 19.2
+// against 20.7; 16 such heads of 1000 tokens, which do not fit: 12.5 against 11.6.
+struct OneKernel {
+  int span;     // logits per row in a CTA's shared memory; 0: not this form
+  size_t smem;
+};
+inline OneKernel one_kernel(int R, int Hkv, int D, const ScoredPlan &pl, int num_sms) {
+  const int tiles = (pl.lp / kTile + kCluster * kCWarps - 1) / (kCluster * kCWarps);
+  if (pl.blocks > 1 || tiles > kCTiles) return {0, 0};
+  const int span = kCWarps * tiles * kTile;
+  const size_t smem = 4 * ((size_t)kCWarps * pl.block * D + (size_t)pl.rows * span);
+  const int resident = D == 64 && smem <= 90 * 1024 ? 2 : 1;
+  if ((long long)R * Hkv * kCluster * 4 > 3ll * num_sms * resident + 8) return {0, 0};
+  return {span, smem};
+}
+
 template <typename T, int D>
 int run_scored(const ScoredArgs &a, const ScoredPlan &pl, cudaStream_t st) {
+  if (const OneKernel one = one_kernel(a.R, a.Hkv, D, pl, a.num_sms); one.span > 0) {
+    auto *k = pl.block == 8 ? scored_cluster_kernel<T, D, 8> : scored_cluster_kernel<T, D, 16>;
+    if (one.smem > 8 * 1024 &&
+        cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             4 * (kCWarps * 16 * D + 16 * kCWarps * kCTiles * kTile)) != cudaSuccess)
+      return -4;
+    return launch_cluster(k, dim3(kCluster, a.Hkv, a.R), dim3(kCWarps * 32), kCluster, one.smem, st, a, pl.rows, one.span);
+  }
   auto *split = pl.block == 8 ? scored_split_kernel<T, D, 8> : scored_split_kernel<T, D, 16>;
   launch_pdl(split, dim3(pl.grid), dim3(kWarps * 32), 0, st, a, pl);
   if (cudaPeekAtLastError() != cudaSuccess) return -4;
-  const int o_ctas = (pl.rows + kJoinRows - 1) / kJoinRows;
-  launch_pdl(scored_join_kernel<T, D>, dim3(o_ctas + (a.max_len + pl.join - 1) / pl.join, a.Hkv, a.R),
-             dim3(kJoin), (size_t)(pl.rows + 4 * kJoin) * sizeof(float), st, a, pl, o_ctas);
+  const int o_ctas = (pl.rows + pl.o_rows - 1) / pl.o_rows;
+  launch_pdl(scored_join_kernel<T, D>, dim3(o_ctas + (a.max_len + pl.join - 1) / pl.join, a.Hkv, a.R), dim3(kJoin),
+             (size_t)(pl.rows + 4 * kJoin) * sizeof(float), st, a, pl, o_ctas);
   return launched();
 }
 }  // namespace kvb
+
+extern "C" long long sched_attn_scored_ws_floats(int R, int Q, int Hq, int Hkv, int D, int max_len, int num_sms) {
+  if (R <= 0 || Q <= 0 || Hkv <= 0 || Hq < Hkv || max_len <= 0) return 0;
+  const kvb::ScoredPlan pl = kvb::scored_plan(R, Q, Hq, Hkv, D, max_len, num_sms);
+  return kvb::one_kernel(R, Hkv, D, pl, num_sms).span > 0 ? 0 : pl.total;
+}
 
 extern "C" int sched_attn_scored(const ScoredArgs *args, cudaStream_t st) {
   if (args == nullptr) return -1;
@@ -987,19 +1326,16 @@ extern "C" int sched_attn_scored(const ScoredArgs *args, cudaStream_t st) {
   const kvb::ScoredPlan pl = kvb::scored_plan(a.R, a.Q, a.Hq, a.Hkv, a.D, a.max_len, a.num_sms);
   // the tile list is indexed in 32 bits (2^31 tiles are 2^35 cached tokens and heads)
   if ((long long)a.R * a.Hkv * pl.blocks * (pl.lp / kvb::kTile) > 0x7fffffffll) return -1;
-  if (a.ws == nullptr || a.ws_floats < pl.total) return -2;
+  if (kvb::one_kernel(a.R, a.Hkv, a.D, pl, a.num_sms).span == 0 && (a.ws == nullptr || a.ws_floats < pl.total)) return -2;
   if (a.element == kKvFp16)
     return a.D == 128 ? kvb::run_scored<__half, 128>(a, pl, st) : kvb::run_scored<__half, 64>(a, pl, st);
   return a.D == 128 ? kvb::run_scored<__nv_bfloat16, 128>(a, pl, st) : kvb::run_scored<__nv_bfloat16, 64>(a, pl, st);
 }
 
-// [R * Hkv] counts, [R * Hkv][2][list] mover and hole slots, and the keys of
-// contexts that shared memory does not hold
-extern "C" long long sched_kv_evict_ws_ints(int R, int Hkv, int max_len, int budget) {
-  if (R <= 0 || Hkv <= 0 || max_len <= budget) return 0;
-  const long long heads = (long long)R * Hkv;
-  const long long list = budget < max_len - budget ? budget : max_len - budget;
-  return heads * (1 + 2 * list + (max_len > kvb::kKeySmem ? max_len : 0));
+// the keys and flags of contexts that shared memory does not hold, for each CTA
+extern "C" long long sched_kv_evict_ws_ints(int R, int Hkv, int max_len, int budget, int num_sms) {
+  if (R <= 0 || Hkv <= 0 || max_len <= budget || max_len <= kvb::kKeySmem) return 0;
+  return (long long)R * Hkv * kvb::evict_plan(R, Hkv, max_len, budget, num_sms).cluster * (long long)kvb::evict_words(max_len);
 }
 
 extern "C" int sched_kv_evict(const KvEvictArgs *args, cudaStream_t st) {
@@ -1009,23 +1345,20 @@ extern "C" int sched_kv_evict(const KvEvictArgs *args, cudaStream_t st) {
   if (a.Hkv < 1 || (a.D != 64 && a.D != 128) || a.page_size < 1 || a.num_pages < 1 || a.bt_pages < 1) return -1;
   if (a.budget < 1 || a.recent < 0 || a.sink < 0 || (long long)a.recent + a.sink > a.budget || a.max_len < 1) return -1;
   if (a.R > 65535 || a.Hkv > 65535 || !aligned16(a.k_cache) || !aligned16(a.v_cache)) return -1;
-  const int list = a.budget < a.max_len - a.budget ? a.budget : a.max_len - a.budget;
-  const long long need = sched_kv_evict_ws_ints(a.R, a.Hkv, a.max_len, a.budget);
+  if ((long long)a.num_pages * a.Hkv * a.page_size >= 0xffffffffll) return -1;  // rows are numbered in 32 bits
+  const long long need = sched_kv_evict_ws_ints(a.R, a.Hkv, a.max_len, a.budget, a.num_sms);
   if (need > 0 && (a.ws == nullptr || a.ws_ints < need)) return -2;
-  const long long heads = (long long)a.R * a.Hkv;
-  int32_t *keys = a.max_len > kvb::kKeySmem ? a.ws + heads * (1 + 2ll * list) : nullptr;
-  const size_t smem = keys == nullptr ? (size_t)a.max_len * 4 : 0;
-  if (smem + sizeof(uint32_t) * (kvb::kSelBins + 64) > 48 * 1024 &&
-      cudaFuncSetAttribute(kvb::evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kvb::kKeySmem * 4) !=
-          cudaSuccess)
+  const kvb::EvictPlan p = kvb::evict_plan(a.R, a.Hkv, a.max_len, a.budget, a.num_sms);
+  auto *k = a.D == 128 ? kvb::evict_kernel<128> : kvb::evict_kernel<64>;
+  const size_t smem = need == 0 && a.max_len > a.budget ? kvb::evict_words(a.max_len) * 4 : 0;
+  if (smem > 24 * 1024 &&
+      cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kvb::evict_words(kvb::kKeySmem) * 4) != cudaSuccess)
     return -4;
-  launch_pdl(kvb::evict_select_kernel, dim3(a.Hkv, a.R), dim3(kvb::kSelThreads), smem, st, a, list, keys);
-  if (cudaPeekAtLastError() != cudaSuccess) return -4;
-  if (a.max_len <= a.budget) return 0;
-  int x = (list + 255) / 256;
-  const long long want = (4ll * a.num_sms + heads - 1) / heads;
-  if (x > want) x = (int)want;
-  auto *mv = a.D == 128 ? kvb::evict_move_kernel<128> : kvb::evict_move_kernel<64>;
-  launch_pdl(mv, dim3(x < 1 ? 1 : x, a.Hkv, a.R), dim3(256), 0, st, a, list);
-  return launched();
+  // vectors of four slots where pages hold whole ones
+  const int vec = a.page_size % 4 == 0 && aligned16(a.scores) && aligned16(a.positions) && aligned16(a.ws);
+  int shift = -1;  // log2 of the page size where it is a power of two
+  if ((a.page_size & (a.page_size - 1)) == 0)
+    for (shift = 0; (1 << shift) < a.page_size;) ++shift;
+  return launch_cluster(k, dim3(p.cluster, a.Hkv, a.R), dim3(p.threads), p.cluster, smem, st, a,
+                        need > 0 ? reinterpret_cast<uint32_t *>(a.ws) : nullptr, vec, shift);
 }

@@ -64,5 +64,5 @@ struct KvEvictArgs {
   long long ws_ints;
   int *status;
 };
-extern "C" long long sched_kv_evict_ws_ints(int R, int Hkv, int max_len, int budget);
+extern "C" long long sched_kv_evict_ws_ints(int R, int Hkv, int max_len, int budget, int num_sms);
 extern "C" int sched_kv_evict(const KvEvictArgs *args, cudaStream_t st);

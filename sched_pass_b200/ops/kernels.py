@@ -218,8 +218,10 @@ def attention_decode(q, out, k_cache, v_cache, block_table, items, num_items, sm
 
 
 def _status_of(t: torch.Tensor) -> torch.Tensor | None:
-    # a CPU tensor is refused by the binding, with its name
-    return status_buffer(t.device) if t.is_cuda else None
+    if not t.is_cuda:
+        return None  # the binding refuses it, by name
+    s = _status.get(t.get_device())
+    return s if s is not None else status_buffer(t.device)
 
 
 def qk_norm_rope_kv_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float,
@@ -265,9 +267,7 @@ def attention_decode_scored(q: torch.Tensor, out: torch.Tensor, k_cache: torch.T
     The pages of one call's requests should be distinct: in a page that two
     requests share, both add their weights, in no fixed order. Pages outside
     the cache are reported and left out."""
-    q4, o4 = (q.unsqueeze(1), out.unsqueeze(1)) if q.dim() == 3 and out.dim() == 3 else (q, out)
-    l3 = lse.unsqueeze(1) if lse is not None and q.dim() == 3 and lse.dim() == 2 else lse
-    ext().attn_decode_scored(q4, o4, k_cache, v_cache, block_table, kv_lens, float(sm_scale), scores, l3, int(max_len),
+    ext().attn_decode_scored(q, out, k_cache, v_cache, block_table, kv_lens, float(sm_scale), scores, lse, int(max_len),
                              _status_of(k_cache))
     return out
 
@@ -293,7 +293,7 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     a prefix cache). Pages outside the cache are reported; their tokens go
     first and are not moved."""
     if new_lens is None:
-        new_lens = torch.empty(kv_lens.shape[0] if kv_lens.dim() else 0, dtype=torch.int32, device=kv_lens.device)
+        new_lens = torch.empty_like(kv_lens)
     ext().kv_evict(k_cache, v_cache, scores, positions, block_table, kv_lens, last_pos, int(budget), int(recent),
                    int(sink), new_lens, int(max_len), _status_of(k_cache))
     return new_lens
