@@ -812,6 +812,7 @@ void qk_norm_rope_kv_append(const at::Tensor &qkv, const at::Tensor &wq, const a
   a.page_size = k_cache.size(2);
   a.num_pages = k_cache.size(0);
   a.element = kv_element(k_cache, "k_cache");
+  a.num_sms = num_sms(k_cache);
   a.status = ptr_or_null<int>(status);
   int rc_ = 0;
   {  // the guard is gone before check_rc may throw

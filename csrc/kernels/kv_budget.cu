@@ -67,6 +67,45 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
 }
 
+// Two fp32 values in one register pair: sm_100 multiplies and adds them at once.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 parts(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void unpack_f2(const uint4 &u, F2 (&f)[4]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 x = unpack2<T>(w[j]);
+    f[j] = f2(x.x, x.y);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack_f2(const F2 (&f)[4]) {
+  const float2 a = parts(f[0]), b = parts(f[1]), c = parts(f[2]), d = parts(f[3]);
+  return make_uint4(pack2<T>(a.x, a.y), pack2<T>(b.x, b.y), pack2<T>(c.x, c.y), pack2<T>(d.x, d.y));
+}
+
 // ------------------------------------------------------------------ norm + rotation + append
 // y = x / sqrt(mean(x^2) + eps) * w over a head's D values, then the first
 // rot values turn in pairs (d, d + rot/2). All in fp32, rounded once.
@@ -74,89 +113,204 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 // D/16 lanes share a head: each holds the two 8-value chunks whose values
 // pair up (chunks l and l + rot/16; lanes behind the rotated part hold the
 // unrotated chunks 2l and 2l + 1), so the rotation needs no exchange and
-// every access is a 16-byte vector. The grid is flat over (token, head).
-template <typename T, int D>
-__global__ void __launch_bounds__(256) qk_norm_kernel(const QkNormArgs a) {
-  constexpr int LANES = D / 16;
-  ptx::pdl_launch_dependents();
-  ptx::pdl_wait();
-  const int nheads = a.Hq + 2 * a.Hkv;
-  const long long items = (long long)a.T * nheads;
-  long long item = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
-  const bool live = item < items;
-  if (!live) item = items - 1;  // takes part in the warp's shuffles, writes nothing
-  const int t = (int)(item / nheads), h = (int)(item - (long long)t * nheads);
-  const int l = threadIdx.x % LANES;
-  const int nr = a.rot / 16;
-  const int c0 = l < nr ? l : 2 * l, c1 = l < nr ? l + nr : 2 * l + 1;
-  const T *src = static_cast<const T *>(a.qkv) + (size_t)t * a.ld_qkv + (size_t)h * D;
-  uint4 u0 = *reinterpret_cast<const uint4 *>(src + c0 * 8);
-  uint4 u1 = *reinterpret_cast<const uint4 *>(src + c1 * 8);
-  const int p = a.pos[t];
-  int s = a.slot[t];
-  const bool pos_ok = p >= 0 && p < a.max_pos;
-  const bool slot_ok = (long long)s < (long long)a.num_pages * a.page_size;
-  if (live && h == 0 && l == 0) {
-    if (!pos_ok)
-      report_bad_index(a.status, kSiteNormPos, p);
-    else if (!slot_ok)
-      report_bad_index(a.status, kSiteKvSlot, s);
-  }
-  if (!slot_ok || !pos_ok) s = -1;  // no cache write
-  if (h < a.Hq + a.Hkv) {
-    float x0[8], x1[8];
-    unpack8<T>(u0, x0);
-    unpack8<T>(u1, x1);
-    float ss = 0.f;
+// every access is a 16-byte vector. A lane group takes NH heads of one kind of
+// a token, all requested at once; weight times cos and sin are theirs in
+// common. PIPE: the grid is resident at once and strides over the groups, and
+// each lane copies its own chunks of the group after next to shared memory
+// meanwhile (cp.async: it takes no registers, and nobody else reads them, so
+// there is no barrier). Otherwise every lane group takes one group.
+constexpr int kNormThreads = 128;
+constexpr int kNormStages = 2;
+constexpr int kNormResident = 5;  // CTAs per SM
+
+__device__ __forceinline__ void cp_async16(void *dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(void *dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(ptx::smem_u32(dst)), "l"(src) : "memory");
+}
+
+template <typename T, int D, int NH, bool PIPE>
+__global__ void __launch_bounds__(kNormThreads, PIPE ? kNormResident : 6) qk_norm_kernel(const QkNormArgs a) {
+  constexpr int LANES = D / 16, ST = PIPE ? kNormStages : 1, BUF = PIPE ? kNormThreads : 1;
+  __shared__ uint4 buf[ST][2 * NH][BUF];
+  __shared__ int32_t where[ST][2][BUF];  // position, slot
+  const int tid = threadIdx.x, l = tid % LANES, nr = a.rot / 16;
+  const int c0 = (l < nr ? l : 2 * l) * 8, c1 = (l < nr ? l + nr : 2 * l + 1) * 8;
+  const uint32_t gq = (a.Hq + NH - 1) / NH, gk = (a.Hkv + NH - 1) / NH, ng = gq + 2 * gk;
+  const uint32_t groups = (uint32_t)a.T * ng, stride = gridDim.x * (kNormThreads / LANES);
+  struct Group {
+    uint32_t t;
+    int kind, h0, heads;  // 0 q, 1 k, 2 v; first head of its kind; number of heads
+    const T *src;
+  };
+  auto group_of = [&](uint32_t i) {
+    Group g;
+    g.t = i / ng;
+    uint32_t r = i - g.t * ng;
+    g.kind = r < gq ? 0 : r < gq + gk ? 1 : 2;
+    r -= g.kind == 0 ? 0 : g.kind == 1 ? gq : gq + gk;
+    g.h0 = (int)r * NH;
+    g.heads = min(NH, (g.kind == 0 ? a.Hq : a.Hkv) - g.h0);
+    g.src = static_cast<const T *>(a.qkv) + (size_t)g.t * a.ld_qkv +
+            (size_t)(g.h0 + (g.kind == 0 ? 0 : g.kind == 1 ? a.Hq : a.Hq + a.Hkv)) * D;
+    return g;
+  };
+  auto request = [&](uint32_t i, int stage) {
+    if (i < groups) {
+      const Group g = group_of(i);
+      cp_async4(&where[stage][0][tid], a.pos + g.t);
+      cp_async4(&where[stage][1][tid], a.slot + g.t);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss += x0[j] * x0[j] + x1[j] * x1[j];
-    // the lanes of a head are aligned neighbours and take this branch together
-    const unsigned mask = (LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u)) << (ptx::lane_id() / LANES * LANES);
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-    const float inv = rsqrtf(ss / (float)D + a.eps);
-    const T *w = static_cast<const T *>(h < a.Hq ? a.wq : a.wk);
-    float w0[8], w1[8];
-    unpack8<T>(*reinterpret_cast<const uint4 *>(w + c0 * 8), w0);
-    unpack8<T>(*reinterpret_cast<const uint4 *>(w + c1 * 8), w1);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x0[j] *= inv * w0[j];
-      x1[j] *= inv * w1[j];
-    }
-    if (l < nr && pos_ok) {
-      const float4 *cs = reinterpret_cast<const float4 *>(a.cos_sin + ((size_t)p * (a.rot / 2) + l * 8) * 2);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4 v = cs[j];  // (cos, sin) of two pairs
-        const float a0 = x0[2 * j], b0 = x1[2 * j], a1 = x0[2 * j + 1], b1 = x1[2 * j + 1];
-        x0[2 * j] = a0 * v.x - b0 * v.y;
-        x1[2 * j] = b0 * v.x + a0 * v.y;
-        x0[2 * j + 1] = a1 * v.z - b1 * v.w;
-        x1[2 * j + 1] = b1 * v.z + a1 * v.w;
+      for (int k = 0; k < NH; ++k) {
+        if (k < g.heads) {
+          cp_async16(&buf[stage][2 * k][tid], g.src + k * D + c0);
+          cp_async16(&buf[stage][2 * k + 1][tid], g.src + k * D + c1);
+        }
       }
     }
-    u0 = pack8<T>(x0);
-    u1 = pack8<T>(x1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  ptx::pdl_launch_dependents();
+  ptx::pdl_wait();
+  uint32_t idx = (blockIdx.x * (uint32_t)kNormThreads + tid) / LANES;
+  if constexpr (PIPE) {
+#pragma unroll
+    for (int st = 0; st < ST; ++st) request(idx + st * stride, st);
   }
-  if (!live) return;
-  T *dst;
-  if (h < a.Hq) {
-    if (!pos_ok) u0 = u1 = make_uint4(0, 0, 0, 0);
-    dst = static_cast<T *>(a.q_out) + (size_t)t * a.ld_q + (size_t)h * D;
-  } else {
-    if (s < 0) return;
-    const int kvh = h < a.Hq + a.Hkv ? h - a.Hq : h - a.Hq - a.Hkv;
-    const int page = s / a.page_size;
-    const size_t row = ((size_t)page * a.Hkv + kvh) * a.page_size + (s - page * a.page_size);
-    dst = static_cast<T *>(h < a.Hq + a.Hkv ? a.k_cache : a.v_cache) + row * D;
-    if (l == 0 && h < a.Hq + a.Hkv) {
-      if (a.scores != nullptr) a.scores[row] = 0.f;
-      if (a.positions != nullptr) a.positions[row] = p;
+  for (int stage = 0; idx < groups; idx += stride, stage = stage + 1 == ST ? 0 : stage + 1) {  // whole lane groups
+    const Group g = group_of(idx);
+    uint4 u0[NH], u1[NH];
+    int p, s;
+    if constexpr (PIPE) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+      p = where[stage][0][tid];
+      s = where[stage][1][tid];
+#pragma unroll
+      for (int i = 0; i < NH; ++i) u0[i] = buf[stage][2 * i][tid], u1[i] = buf[stage][2 * i + 1][tid];
+      request(idx + ST * stride, stage);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NH; ++i) {
+        if (i < g.heads) {
+          u0[i] = *reinterpret_cast<const uint4 *>(g.src + i * D + c0);
+          u1[i] = *reinterpret_cast<const uint4 *>(g.src + i * D + c1);
+        }
+      }
+      p = a.pos[g.t];
+      s = a.slot[g.t];
+    }
+    const bool pos_ok = (uint32_t)p < (uint32_t)a.max_pos;
+    const bool slot_ok = s < 0 || (long long)s < (long long)a.num_pages * a.page_size;
+    if (g.kind == 0 && g.h0 == 0 && l == 0) {
+      if (!pos_ok)
+        report_bad_index(a.status, kSiteNormPos, p);
+      else if (!slot_ok)
+        report_bad_index(a.status, kSiteKvSlot, s);
+    }
+    if (!slot_ok || !pos_ok) s = -1;  // no cache write
+    if (g.kind < 2) {
+      F2 w0[4], w1[4];
+      const T *w = static_cast<const T *>(g.kind == 0 ? a.wq : a.wk);
+      unpack_f2<T>(*reinterpret_cast<const uint4 *>(w + c0), w0);
+      unpack_f2<T>(*reinterpret_cast<const uint4 *>(w + c1), w1);
+      // y0 = x0 (w0 cos) - x1 (w1 sin), y1 = x1 (w1 cos) + x0 (w0 sin)
+      F2 s0[4], s1[4];
+      const bool turns = l < nr;
+      if (turns) {
+        const float4 *cs = reinterpret_cast<const float4 *>(a.cos_sin + ((size_t)(pos_ok ? p : 0) * (a.rot / 2) + l * 8) * 2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float4 v = cs[j];  // (cos, sin) of two pairs
+          const F2 c = f2(v.x, v.z), sn = f2(v.y, v.w), ns = f2(-v.y, -v.w);
+          s0[j] = w1[j] * ns;
+          s1[j] = w0[j] * sn;
+          w0[j] = w0[j] * c;
+          w1[j] = w1[j] * c;
+        }
+      }
+      // the lanes of a head are aligned neighbours with the same number of heads
+      const unsigned mask = ((1u << LANES) - 1u) << (ptx::lane_id() / LANES * LANES);
+#pragma unroll
+      for (int i = 0; i < NH; ++i) {
+        if (i >= g.heads) break;
+        F2 x0[4], x1[4], q = f2(0.f, 0.f);
+        unpack_f2<T>(u0[i], x0);
+        unpack_f2<T>(u1[i], x1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q = fma2(x1[j], x1[j], fma2(x0[j], x0[j], q));
+        float ss = parts(q).x + parts(q).y;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+        const float inv = rsqrtf(ss * (1.f / D) + a.eps);
+        const F2 iv = f2(inv, inv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x0[j] = x0[j] * iv;
+          x1[j] = x1[j] * iv;
+          const F2 y0 = x0[j] * w0[j], y1 = x1[j] * w1[j];
+          if (turns) {
+            const F2 z0 = fma2(x1[j], s0[j], y0);
+            x1[j] = fma2(x0[j], s1[j], y1);
+            x0[j] = z0;
+          } else {
+            x0[j] = y0;
+            x1[j] = y1;
+          }
+        }
+        u0[i] = pack_f2<T>(x0);
+        u1[i] = pack_f2<T>(x1);
+      }
+    }
+    T *dst;
+    size_t pitch = D;
+    if (g.kind == 0) {
+      dst = static_cast<T *>(a.q_out) + (size_t)g.t * a.ld_q + (size_t)g.h0 * D;
+      if (!pos_ok) {
+#pragma unroll
+        for (int i = 0; i < NH; ++i) u0[i] = u1[i] = make_uint4(0, 0, 0, 0);
+      }
+    } else {
+      if (s < 0) continue;
+      const int page = s / a.page_size;
+      const size_t row = ((size_t)page * a.Hkv + g.h0) * a.page_size + (s - page * a.page_size);
+      pitch = (size_t)a.page_size * D;
+      dst = static_cast<T *>(g.kind == 1 ? a.k_cache : a.v_cache) + row * D;
+      if (g.kind == 1) {
+        for (int i = l; i < g.heads; i += LANES) {
+          if (a.scores != nullptr) a.scores[row + (size_t)i * a.page_size] = 0.f;
+          if (a.positions != nullptr) a.positions[row + (size_t)i * a.page_size] = p;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NH; ++i) {
+      if (i < g.heads) {
+        *reinterpret_cast<uint4 *>(dst + i * pitch + c0) = u0[i];
+        *reinterpret_cast<uint4 *>(dst + i * pitch + c1) = u1[i];
+      }
     }
   }
-  *reinterpret_cast<uint4 *>(dst + c0 * 8) = u0;
-  *reinterpret_cast<uint4 *>(dst + c1 * 8) = u1;
+}
+
+// Heads per lane group, by the lanes that one head each would take per SM.
+// Measured with 32 + 8 heads of 128, bf16, cold tensors: 256 tokens (664 lanes)
+// 3.4 us with one head, 3.6 with two, 4.5 with four in the pipeline; 1024
+// tokens 8.6, 6.6, 7.3; 4097 tokens 31, 25.6, 22.7; 8000 tokens 64, 47, 37
+// (5.4 TB/s; copying as many bytes takes 18 us for 4097 tokens, 33 for 8000).
+template <typename T, int D>
+int run_qk_norm(const QkNormArgs &a, cudaStream_t st) {
+  const long long lanes = (long long)a.T * (a.Hq + 2 * a.Hkv) * (D / 16);
+  const int nh = lanes <= 768ll * a.num_sms ? 1 : lanes <= 4096ll * a.num_sms ? 2 : 4;
+  const long long groups = (long long)a.T * ((a.Hq + nh - 1) / nh + 2ll * ((a.Hkv + nh - 1) / nh));
+  const long long need = (groups * (D / 16) + kNormThreads - 1) / kNormThreads, most = (long long)a.num_sms * kNormResident;
+  if (groups + (kNormStages + 1) * most * kNormThreads > 0xffffffffll) return -1;  // groups are numbered in 32 bits
+  const long long grid = nh < 4 || need < most ? need : most;
+  launch_pdl(nh == 1   ? qk_norm_kernel<T, D, 1, false>
+             : nh == 2 ? qk_norm_kernel<T, D, 2, false>
+                       : qk_norm_kernel<T, D, 4, true>,
+             dim3((unsigned)grid), dim3(kNormThreads), 0, st, a);
+  return cudaPeekAtLastError() == cudaSuccess ? 0 : -4;
 }
 
 // ------------------------------------------------------------------ scored decode attention
@@ -1248,23 +1402,15 @@ extern "C" int sched_qk_norm_rope_kv_append(const QkNormArgs *args, cudaStream_t
   if (args == nullptr) return -1;
   const QkNormArgs &a = *args;
   if (a.T <= 0) return 0;
-  const int nheads = a.Hq + 2 * a.Hkv;
   if (a.Hq < 1 || a.Hkv < 1 || a.page_size < 1 || a.num_pages < 1 || a.max_pos < 1) return -1;
   if ((a.D != 64 && a.D != 128) || a.rot < 16 || a.rot > a.D || a.rot % 16 != 0) return -1;
   if (a.ld_qkv % 8 != 0 || a.ld_q % 8 != 0) return -1;
   if (!aligned16(a.qkv) || !aligned16(a.wq) || !aligned16(a.wk) || !aligned16(a.cos_sin) || !aligned16(a.q_out) ||
       !aligned16(a.k_cache) || !aligned16(a.v_cache))
     return -1;
-  const long long threads = (long long)a.T * nheads * (a.D / 16);
-  const long long grid = (threads + 255) / 256;
-  if (grid > 0x7fffffffll) return -1;
-  auto *k = a.element == kKvFp16 ? (a.D == 128 ? kvb::qk_norm_kernel<__half, 128> : kvb::qk_norm_kernel<__half, 64>)
-                                 : (a.D == 128 ? kvb::qk_norm_kernel<__nv_bfloat16, 128>
-                                               : kvb::qk_norm_kernel<__nv_bfloat16, 64>);
-  launch_pdl(k, dim3((unsigned)grid), dim3(256), 0, st, a);
-  return launched();
+  if (a.element == kKvFp16) return a.D == 128 ? kvb::run_qk_norm<__half, 128>(a, st) : kvb::run_qk_norm<__half, 64>(a, st);
+  return a.D == 128 ? kvb::run_qk_norm<__nv_bfloat16, 128>(a, st) : kvb::run_qk_norm<__nv_bfloat16, 64>(a, st);
 }
-
 
 namespace kvb {
 // The one-kernel form, for a few tiles a warp and clusters that are all

@@ -22,7 +22,7 @@ struct QkNormArgs {
   void *k_cache, *v_cache;  // [num_pages, Hkv, page_size, D]
   float *scores;            // [num_pages, Hkv, page_size] or null: set to 0 at the new slots
   int32_t *positions;       // the same shape or null: set to the position
-  int T, Hq, Hkv, D, page_size, num_pages, element;
+  int T, Hq, Hkv, D, page_size, num_pages, element, num_sms;
   int *status;
 };
 extern "C" int sched_qk_norm_rope_kv_append(const QkNormArgs *args, cudaStream_t st);

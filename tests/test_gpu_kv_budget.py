@@ -136,6 +136,14 @@ def test_append_small_and_large_rows(scale):
     check_append(9, 4, 2, 128, 128, BF, scale=scale, zero_head=True)
 
 
+@pytest.mark.parametrize("T,Hq,Hkv,D,rot,dtype", [
+    (700, 8, 3, 128, 128, BF), (2600, 7, 2, 128, 64, FP), (3100, 5, 1, 64, 64, BF), (9001, 15, 3, 64, 32, FP)])
+def test_append_many_tokens(T, Hq, Hkv, D, rot, dtype):
+    """The forms for more tokens: several heads to a lane group, with and
+    without the pipeline, head counts that do not fill the last group."""
+    check_append(T, Hq, Hkv, D, rot, dtype, seed=T)
+
+
 def test_append_no_tokens():
     check_append(0, 4, 2, 64, 64, BF)
 
