@@ -856,7 +856,7 @@ void attn_decode_scored(const at::Tensor &q, at::Tensor &out, const at::Tensor &
   TORCH_CHECK(max_len >= 0, "max_len must not be negative");
   int64_t cap = block_table.size(1) * ps;
   if (max_len > 0 && max_len < cap) cap = max_len;
-  TORCH_CHECK(cap <= INT32_MAX - 1024, "contexts of 2^31 tokens or more");
+  TORCH_CHECK(cap < (1 << 30), "contexts of 2^30 tokens or more");
   check_cuda(k_cache, "k_cache");
   const std::pair<const at::Tensor *, const char *> on[] = {{&q, "q"}, {&out, "out"}, {&v_cache, "v_cache"},
       {&block_table, "block_table"}, {&kv_lens, "kv_lens"}, {&scores, "scores"}};
@@ -930,7 +930,7 @@ void kv_evict(at::Tensor &k_cache, at::Tensor &v_cache, at::Tensor &scores, at::
   TORCH_CHECK(max_len >= 0, "max_len must not be negative");
   int64_t cap = block_table.size(1) * ps;
   if (max_len > 0 && max_len < cap) cap = max_len;
-  TORCH_CHECK(cap <= INT32_MAX - 1024, "contexts of 2^31 tokens or more");
+  TORCH_CHECK(cap < (1 << 30), "contexts of 2^30 tokens or more");
   check_cuda(k_cache, "k_cache");
   const std::pair<const at::Tensor *, const char *> on[] = {{&v_cache, "v_cache"}, {&scores, "scores"},
       {&positions, "positions"}, {&block_table, "block_table"}, {&kv_lens, "kv_lens"}, {&last_pos, "last_pos"},

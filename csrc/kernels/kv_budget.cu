@@ -1046,7 +1046,7 @@ __global__ void __launch_bounds__(kJoin, 4) scored_join_kernel(const ScoredArgs 
 // < budget of evicted ones, the i-th the i-th: sources and destinations are
 // disjoint, so the moves need no order and only they touch K and V.
 constexpr int kBins = 2048;          // of a selection digit: 11, 11 and 10 bits
-constexpr int kFew = 256;            // keys that one warp finishes the selection of, eight a lane
+constexpr int kFew = 256;            // keys that are ranked by comparing all pairs, a thread each
 constexpr int kWindow = 1024;        // moves a CTA lists at a time
 constexpr int kKeySmem = 40 * 1024;  // slots whose keys fit shared memory; longer contexts keep them in the workspace
 constexpr uint32_t kNoRow = 0xffffffffu;
@@ -1067,9 +1067,9 @@ __device__ __forceinline__ uint32_t warp_scan(uint32_t v) {  // inclusive
   return v;
 }
 
-// Words a CTA needs for n slots: a key each, and a flag word and its prefix
-// for every 32; a multiple of 16 bytes, so that every CTA's keys start on one.
-__host__ __device__ __forceinline__ size_t evict_words(int n) { return ((size_t)((n + 31) / 32) * (32 + 2) + 3) / 4 * 4; }
+// Words a CTA needs for n slots: for every block of 128 a key each and four
+// flag words (bit l of word e: slot 4 l + e); multiples of 16 bytes.
+__host__ __device__ __forceinline__ size_t evict_words(int n) { return (size_t)((n + 127) / 128) * (128 + 4); }
 
 // A cluster has a (request, KV head). Every CTA of it finds the budget-th
 // largest key by radix selection over all the keys (8 bytes a token to read;
@@ -1080,9 +1080,9 @@ __host__ __device__ __forceinline__ size_t evict_words(int n) { return ((size_t)
 // slot. A flag marks the slots below the budget that lose their token and the
 // slots behind it that keep theirs; as many of the one as of the other, so one
 // prefix sum over the flags ranks both.
-template <int D>
+template <int D, bool IN_WS>
 __global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32_t *ws, int vec, int page_shift) {
-  extern __shared__ __align__(16) uint32_t dyn[];  // evict_words(max_len) unless they are in the workspace
+  extern __shared__ __align__(16) uint32_t dyn[];  // evict_words(max_len) unless they are in the workspace (IN_WS)
   __shared__ __align__(16) uint32_t hist[kBins];
   __shared__ uint32_t tot[32], s_bin, s_above, s_count, s_found, s_key;
   __shared__ int s_slot;
@@ -1101,9 +1101,13 @@ __global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32
   if (n <= b) return;  // the whole cluster
   const int32_t *bt = a.block_table + (size_t)req * a.bt_stride;
   const int after = (int)max((long long)a.last_pos[req] - a.recent, -0x80000000ll);
-  uint32_t *keys = ws == nullptr ? dyn : ws + (((size_t)req * a.Hkv + h) * C + rank) * evict_words(a.max_len);
-  const int nw = (n + 31) / 32;
-  uint32_t *flags = keys + (size_t)nw * 32, *before = flags + nw;
+  uint32_t *keys;
+  if constexpr (IN_WS)
+    keys = ws + (((size_t)req * a.Hkv + h) * C + rank) * evict_words(a.max_len);
+  else
+    keys = dyn;
+  const int nb = (n + 127) / 128;
+  uint32_t *flags = keys + (size_t)nb * 128;
   // the row of a slot in the cache and in scores / positions, kNoRow for a bad page
   auto row_of = [&](int j) {
     const int col = page_shift >= 0 ? j >> page_shift : j / a.page_size, page = bt[col];
@@ -1165,9 +1169,12 @@ __global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32
     const int shift = digit == 0 ? 21 : (digit == 1 ? 10 : 0);
     const uint32_t top = digit == 2 ? 1023u : 2047u;
     if (digit > 0) {
-      for (int j = tid; j < n; j += NT) {
-        const uint32_t k = keys[j];
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & top], 1u);
+      for (int j = tid * 4; j < n; j += NT * 4) {
+        const uint4 k = *reinterpret_cast<const uint4 *>(keys + j);
+        if ((k.x & mask) == prefix) atomicAdd(&hist[(k.x >> shift) & top], 1u);
+        if ((k.y & mask) == prefix && j + 1 < n) atomicAdd(&hist[(k.y >> shift) & top], 1u);
+        if ((k.z & mask) == prefix && j + 2 < n) atomicAdd(&hist[(k.z >> shift) & top], 1u);
+        if ((k.w & mask) == prefix && j + 3 < n) atomicAdd(&hist[(k.w >> shift) & top], 1u);
       }
     }
     __syncthreads();
@@ -1213,50 +1220,27 @@ __global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32
     const uint32_t match = s_count;
     if (match == need) break;  // all keys that match the digits so far stay: the other digits decide nothing
     if (match <= kFew) {
-      // few keys match: one warp finishes, bit by bit, with the slots of the listed keys for ties
-      for (int j = tid; j < n; j += NT) {
-        const uint32_t k = keys[j];
-        if ((k & mask) == prefix) {
-          const uint32_t i = atomicAdd(&s_found, 1u);
-          from[i] = k;
-          to[i] = (uint32_t)j;
-        }
+      // few keys match: the one that (need - 1) others precede, by key and then slot, is the last kept
+      unsigned long long *few = reinterpret_cast<unsigned long long *>(from);
+      if (tid == 0) few[match] = 0;  // the list is read in pairs
+      for (int j = tid * 4; j < n; j += NT * 4) {
+        const uint4 four = *reinterpret_cast<const uint4 *>(keys + j);
+        const uint32_t k[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((k[e] & mask) == prefix && j + e < n)
+            few[atomicAdd(&s_found, 1u)] = (unsigned long long)k[e] << 32 | (uint32_t)~(j + e);
       }
       __syncthreads();
-      if (warp == 0) {
-        uint32_t k[kFew / 32];
-        int slot[kFew / 32];
-#pragma unroll
-        for (int i = 0; i < kFew / 32; ++i) {
-          const uint32_t at = i * 32 + lane;
-          k[i] = at < match ? from[at] : 0u;  // below any key that matches, or among its equals the last
-          slot[i] = at < match ? (int)to[at] : 0x7fffffff;
+      if (tid < (int)match) {
+        const unsigned long long me = few[tid];
+        uint32_t ahead = 0;
+#pragma unroll 4
+        for (uint32_t i = 0; i < match; i += 2) {
+          const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(few + i);
+          ahead += (two.x > me) + (two.y > me);
         }
-        uint32_t key = prefix, equal = 0, more = 0;  // the largest key with `need` keys not below it
-        for (uint32_t bit = (1u << shift) >> 1; bit != 0; bit >>= 1) {
-          uint32_t c = 0;
-#pragma unroll
-          for (int i = 0; i < kFew / 32; ++i) c += slot[i] != 0x7fffffff && k[i] >= (key | bit);
-          if (__reduce_add_sync(0xffffffffu, c) >= need) key |= bit;
-        }
-#pragma unroll
-        for (int i = 0; i < kFew / 32; ++i) {
-          more += slot[i] != 0x7fffffff && k[i] > key;
-          equal += slot[i] != 0x7fffffff && k[i] == key;
-        }
-        more = __reduce_add_sync(0xffffffffu, more);
-        equal = __reduce_add_sync(0xffffffffu, equal);
-        int upto = 0x7fffffff;
-        if (more + equal > need) {  // of the equal ones, the lowest slots: the smallest bound with enough up to it
-          upto = 0;
-          for (int bit = 1 << (31 - __clz(n)); bit != 0; bit >>= 1) {
-            uint32_t c = 0;
-#pragma unroll
-            for (int i = 0; i < kFew / 32; ++i) c += k[i] == key && slot[i] < (upto | bit);
-            if (__reduce_add_sync(0xffffffffu, c) < need - more) upto |= bit;
-          }
-        }
-        if (lane == 0) s_key = key, s_slot = upto;
+        if (ahead == need - 1) s_key = (uint32_t)(me >> 32), s_slot = (int)~(uint32_t)me;
       }
       __syncthreads();
       prefix = s_key;
@@ -1267,43 +1251,69 @@ __global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32
     if (digit == 2) last_slot = -1;  // many equal keys: found by the prefix sum below
   }
 
-  // Sets flags[w] to the slots j of word w for which f(j, key) holds and
-  // before[w] to the number of such slots in front of it; returns their total.
+  // Of the four slots from j on, a bit for each below `bound`.
+  auto below = [](int j, int bound) { return (1u << min(max(bound - j, 0), 4)) - 1u; };
+  // Sets the flags that f(first of four slots, their keys) gives; returns their number.
   auto flag = [&](auto f) {
-#pragma unroll 4
-    for (int w = warp; w < nw; w += NW) {
-      const int j = w * 32 + lane;
-      const uint32_t word = __ballot_sync(0xffffffffu, j < n && f(j, j < n ? keys[j] & mask : 0u));
-      if (lane == 0) flags[w] = word;
+    uint32_t mine = 0;
+#pragma unroll 2
+    for (int w = warp; w < nb; w += NW) {
+      const int j = w * 128 + lane * 4;
+      const uint4 k = *reinterpret_cast<const uint4 *>(keys + j);
+      const uint32_t four = f(j, make_uint4(k.x & mask, k.y & mask, k.z & mask, k.w & mask)) & below(j, n);
+      uint32_t word = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t all = __ballot_sync(0xffffffffu, four >> e & 1u);
+        mine += __popc(all);
+        if (lane == e) word = all;
+      }
+      if (lane < 4) flags[w * 4 + lane] = word;
     }
+    if (lane == 0) tot[warp] = mine;
     __syncthreads();
-    uint32_t carry = 0;
-    for (int w0 = 0; w0 < nw; w0 += NT) {
-      const uint32_t c = w0 + tid < nw ? __popc(flags[w0 + tid]) : 0;
-      const uint32_t inc = warp_scan(c);
-      if (lane == 31) tot[warp] = inc;
-      __syncthreads();
-      const uint32_t front = warp_scan(lane < NW ? tot[lane] : 0u);
-      const uint32_t warps_ahead = __shfl_sync(0xffffffffu, front, max(warp - 1, 0));
-      if (w0 + tid < nw) before[w0 + tid] = carry + inc - c + (warp > 0 ? warps_ahead : 0u);
-      carry += __shfl_sync(0xffffffffu, front, 31);
-      __syncthreads();
-    }
-    return carry;
+    return __reduce_add_sync(0xffffffffu, lane < NW ? tot[lane] : 0u);
   };
-  if (last_slot < 0) {
-    flag([&](int, uint32_t k) { return k == prefix; });
-    for (int w = tid; w < nw; w += NT) {  // the word with the need-th of them
-      const uint32_t f = flags[w], at = before[w];
-      if (at < need && at + __popc(f) >= need) s_slot = w * 32 + (int)__fns(f, 0, (int)(need - at));
+  // Calls f(j, number of flags in front) for the flagged slots of this warp's
+  // blocks; every warp counts all blocks, 32 at a time, for itself.
+  auto flagged = [&](auto f) {
+    uint32_t front = 0;
+    for (int w0 = 0; w0 < nb; w0 += 32) {
+      uint32_t c = 0;
+      if (w0 + lane < nb) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(flags + (w0 + lane) * 4);
+        c = __popc(v.x) + __popc(v.y) + __popc(v.z) + __popc(v.w);
+      }
+      const uint32_t inc = warp_scan(c);
+      for (int w = w0 + warp; w < min(nb, w0 + 32); w += NW) {
+        if (__shfl_sync(0xffffffffu, c, w - w0) == 0) continue;
+        const uint4 v = *reinterpret_cast<const uint4 *>(flags + w * 4);
+        const uint32_t word[4] = {v.x, v.y, v.z, v.w}, lower = (1u << lane) - 1u;
+        uint32_t at = front + __shfl_sync(0xffffffffu, inc - c, w - w0) + __popc(v.x & lower) + __popc(v.y & lower) +
+                      __popc(v.z & lower) + __popc(v.w & lower);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (word[e] >> lane & 1u) f(w * 128 + lane * 4 + e, at++);
+        }
+      }
+      front += __shfl_sync(0xffffffffu, inc, 31);
     }
+  };
+  auto bits = [](bool a, bool b, bool c, bool d) { return (uint32_t)a | (uint32_t)b << 1 | (uint32_t)c << 2 | (uint32_t)d << 3; };
+  if (last_slot < 0) {
+    flag([&](int, const uint4 &k) { return bits(k.x == prefix, k.y == prefix, k.z == prefix, k.w == prefix); });
+    flagged([&](int j, uint32_t at) {
+      if (at == need - 1) s_slot = j;
+    });
     __syncthreads();
     last_slot = s_slot;
     __syncthreads();
   }
-  const int moves = (int)(flag([&](int j, uint32_t k) {
-                            const bool keep = k > prefix || (k == prefix && j <= last_slot);
-                            return keep == (j >= b);
+  const int upto = min(last_slot, n - 1) + 1;
+  const int moves = (int)(flag([&](int j, const uint4 &k) {
+                            const uint32_t more = bits(k.x > prefix, k.y > prefix, k.z > prefix, k.w > prefix);
+                            const uint32_t same = bits(k.x == prefix, k.y == prefix, k.z == prefix, k.w == prefix);
+                            return (more | (same & below(j, upto))) ^ below(j, b);  // kept and behind the budget, or neither
                           }) / 2);
   if (C > 1) ptx::cluster_sync_all();  // every CTA has read the scores: they may change
 
@@ -1316,16 +1326,12 @@ __global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32
   const int share = (moves + C - 1) / C, r0 = min(moves, rank * share), r1 = min(moves, r0 + share);
   for (int q0 = r0; q0 < r1; q0 += kWindow) {
     const int cnt = min(r1 - q0, kWindow);
-    for (int w = warp; w < nw; w += NW) {
-      const uint32_t word = flags[w];
-      if (word >> lane & 1u) {
-        const int j = w * 32 + lane;
-        int i = (int)(before[w] + __popc(word & ((1u << lane) - 1u))) - q0;
-        uint32_t *list = to;
-        if (j >= b) i -= moves, list = from;
-        if (i >= 0 && i < cnt) list[i] = (uint32_t)j;
-      }
-    }
+    flagged([&](int j, uint32_t at) {
+      int i = (int)at - q0;
+      uint32_t *list = to;
+      if (j >= b) i -= moves, list = from;
+      if (i >= 0 && i < cnt) list[i] = (uint32_t)j;
+    });
     __syncthreads();
     for (int i = tid; i < cnt; i += NT) {  // slots to rows, and the tracking entries
       const uint32_t src = row_of((int)from[i]);
@@ -1465,7 +1471,7 @@ extern "C" int sched_attn_scored(const ScoredArgs *args, cudaStream_t st) {
   if (a.R <= 0 || a.Q <= 0) return 0;
   if (a.Hkv < 1 || a.Hq < a.Hkv || a.Hq % a.Hkv != 0 || (a.D != 64 && a.D != 128)) return -1;
   if (a.page_size < 16 || a.page_size % 16 != 0 || a.num_pages < 1 || a.max_len < 1 || a.bt_pages < 1) return -1;
-  if (a.R > 65535 || a.Hkv > 65535 || (long long)a.Q * (a.Hq / a.Hkv) > 8192) return -1;
+  if (a.R > 65535 || a.Hkv > 65535 || a.max_len >= 1 << 30 || (long long)a.Q * (a.Hq / a.Hkv) > 8192) return -1;
   if (a.q_req % 8 != 0 || a.q_query % 8 != 0 || !aligned16(a.q) || !aligned16(a.k_cache) || !aligned16(a.v_cache) ||
       !aligned16(a.scores) || !aligned16(a.ws))
     return -1;
@@ -1490,12 +1496,13 @@ extern "C" int sched_kv_evict(const KvEvictArgs *args, cudaStream_t st) {
   if (a.R <= 0) return 0;
   if (a.Hkv < 1 || (a.D != 64 && a.D != 128) || a.page_size < 1 || a.num_pages < 1 || a.bt_pages < 1) return -1;
   if (a.budget < 1 || a.recent < 0 || a.sink < 0 || (long long)a.recent + a.sink > a.budget || a.max_len < 1) return -1;
-  if (a.R > 65535 || a.Hkv > 65535 || !aligned16(a.k_cache) || !aligned16(a.v_cache)) return -1;
+  if (a.R > 65535 || a.Hkv > 65535 || a.max_len >= 1 << 30 || !aligned16(a.k_cache) || !aligned16(a.v_cache)) return -1;
   if ((long long)a.num_pages * a.Hkv * a.page_size >= 0xffffffffll) return -1;  // rows are numbered in 32 bits
   const long long need = sched_kv_evict_ws_ints(a.R, a.Hkv, a.max_len, a.budget, a.num_sms);
   if (need > 0 && (a.ws == nullptr || a.ws_ints < need)) return -2;
   const kvb::EvictPlan p = kvb::evict_plan(a.R, a.Hkv, a.max_len, a.budget, a.num_sms);
-  auto *k = a.D == 128 ? kvb::evict_kernel<128> : kvb::evict_kernel<64>;
+  auto *k = need > 0 ? (a.D == 128 ? kvb::evict_kernel<128, true> : kvb::evict_kernel<64, true>)
+                     : (a.D == 128 ? kvb::evict_kernel<128, false> : kvb::evict_kernel<64, false>);
   const size_t smem = need == 0 && a.max_len > a.budget ? kvb::evict_words(a.max_len) * 4 : 0;
   if (smem > 24 * 1024 &&
       cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kvb::evict_words(kvb::kKeySmem) * 4) != cudaSuccess)
