@@ -822,8 +822,9 @@ void qk_norm_rope_kv_append(const at::Tensor &qkv, const at::Tensor &wq, const a
   check_rc(rc_, "qk_norm_rope_kv_append");
 }
 
-// q, out [R, Q, Hq, D] and lse [R, Q, Hq], or without Q for one query
-void attn_decode_scored(const at::Tensor &q, at::Tensor &out, const at::Tensor &k_cache, const at::Tensor &v_cache,
+// q, out [R, Q, Hq, D] and lse [R, Q, Hq], or without Q for one query; returns
+// the number of kernels launched
+int64_t attn_decode_scored(const at::Tensor &q, at::Tensor &out, const at::Tensor &k_cache, const at::Tensor &v_cache,
                         const at::Tensor &block_table, const at::Tensor &kv_lens, double sm_scale, at::Tensor &scores,
                         const c10::optional<at::Tensor> &lse, int64_t max_len, const c10::optional<at::Tensor> &status) {
   check_cache(k_cache, v_cache);
@@ -862,7 +863,7 @@ void attn_decode_scored(const at::Tensor &q, at::Tensor &out, const at::Tensor &
       {&block_table, "block_table"}, {&kv_lens, "kv_lens"}, {&scores, "scores"}};
   for (const auto &t : on) check_on(*t.first, k_cache, t.second);
   if (lse.has_value()) check_on(*lse, k_cache, "lse");
-  if (R == 0 || Q == 0) return;
+  if (R == 0 || Q == 0) return 0;
   check_aligned(q, "q");
   check_aligned(out, "out");
   check_aligned(k_cache, "k_cache");
@@ -907,6 +908,7 @@ void attn_decode_scored(const at::Tensor &q, at::Tensor &out, const at::Tensor &
     rc_ = sched_attn_scored(&a, cur_stream());
   }
   check_rc(rc_, "attn_decode_scored");
+  return a.ws_floats == 0 ? 1 : 2;
 }
 
 void kv_evict(at::Tensor &k_cache, at::Tensor &v_cache, at::Tensor &scores, at::Tensor &positions,

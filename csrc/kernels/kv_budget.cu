@@ -62,11 +62,6 @@ __device__ __forceinline__ void unpack8(const uint4 &u, float (&f)[8]) {
   const float2 a = unpack2<T>(u.x), b = unpack2<T>(u.y), c = unpack2<T>(u.z), d = unpack2<T>(u.w);
   f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y, f[4] = c.x, f[5] = c.y, f[6] = d.x, f[7] = d.y;
 }
-template <typename T>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-}
-
 // Two fp32 values in one register pair: sm_100 multiplies and adds them at once.
 struct F2 {
   uint64_t v;
@@ -329,7 +324,11 @@ int run_qk_norm(const QkNormArgs &a, cudaStream_t st) {
 // list, so (warp + task) numbers the partial results without gaps to look up.
 constexpr int kWarps = 4;      // per CTA of the split kernel
 constexpr int kTile = 16;      // tokens per warp step: divides the page size
-constexpr int kResident = 3;   // CTAs of the split kernel per SM
+// CTAs of the split kernel per SM, by its registers. Measured: 64 requests of
+// 1664 tokens, 8 heads of 128, 4 query rows each 78 us with three, 90 with two,
+// 121 with four (spills); 16 rows 115 with two, 126 with three. 4 heads of 64,
+// 64 x 4000 tokens: 4 rows 61 us with four, 69 with three; 16 rows 85 and 89.
+constexpr int resident(int D, int block) { return D == 64 ? 4 : block == 16 ? 2 : 3; }
 constexpr int kMinRun = 2;     // tiles per warp at least: bounds the partial results
 
 struct ScoredPlan {
@@ -350,11 +349,11 @@ inline ScoredPlan scored_plan(int R, int Q, int Hq, int Hkv, int D, int max_len,
   p.blocks = (p.rows + p.block - 1) / p.block;
   const long long heads = (long long)R * Hkv, tasks = heads * p.blocks;
   const long long most = (tasks * (p.lp / kTile) + kMinRun * kWarps - 1) / (kMinRun * kWarps);
-  const long long fill = (long long)num_sms * kResident;
+  const long long fill = (long long)num_sms * resident(D, p.block);
   p.grid = (int)(most < fill ? most : fill);
   // the join's CTAs all resident at once where that is possible, with each thread having a logit to read
   p.join = p.rows >= 16 ? 64 : p.rows >= 8 ? 128 : p.rows >= 4 ? 256 : p.rows >= 2 ? 512 : 1024;
-  while (heads * ((max_len + p.join - 1) / p.join) > 3ll * num_sms && p.join < max_len) p.join += p.join < 1024 ? p.join : 1024;
+  while (heads * ((max_len + p.join - 1) / p.join) > 4ll * num_sms && p.join < max_len) p.join += p.join < 1024 ? p.join : 1024;
   // and at most 16 partial results per warp
   p.o_rows = 1;
   while (p.o_rows < 8 && heads * ((p.rows + p.o_rows - 1) / p.o_rows) > num_sms && p.grid * kWarps / tasks * p.o_rows * 2 <= 8 * 16)
@@ -645,7 +644,7 @@ struct RowSoftmax {
 
 // One warp: a run of the tile list.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kWarps * 32, kResident)
+__global__ void __launch_bounds__(kWarps * 32, resident(D, ROWS))
     scored_split_kernel(const ScoredArgs a, const ScoredPlan pl) {
   __shared__ typename RowSoftmax<T, D, ROWS>::QTile q_sm[kWarps];
   ptx::pdl_launch_dependents();
@@ -686,6 +685,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident)
   {
     uint32_t before = 0;  // tiles (of one head) in front of request i0
     for (int i0 = 0;; i0 += 32) {
+      if (i0 >= a.R) return;  // only if kv_lens changes under the kernel
       const uint32_t own = i0 + lane < a.R ? tiles_of(checked_len(a.kv_lens[i0 + lane], cap, nullptr, 0, false)) : 0;
       uint32_t inc = own;
 #pragma unroll
@@ -726,8 +726,10 @@ __global__ void __launch_bounds__(kWarps * 32, kResident)
           n_tile = 0;
           if (++n_hb == HB) {
             n_hb = 0;
-            do n_n = checked_len(a.kv_lens[++n_req], cap, nullptr, 0, false);
-            while (n_n == 0);  // more tiles follow, so a request with some does
+            do {  // more tiles follow, so a request with some does
+              if (++n_req >= a.R) return;  // only if kv_lens changes under the kernel
+              n_n = checked_len(a.kv_lens[n_req], cap, nullptr, 0, false);
+            } while (n_n == 0);
           }
         }
         next = tile_base(a, n_req, n_hb / pl.blocks, n_tile * kTile);

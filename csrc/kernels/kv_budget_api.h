@@ -42,7 +42,7 @@ struct ScoredArgs {
   const int32_t *kv_lens;
   int R, Q, Hq, Hkv, D, page_size, num_pages, max_len, element, num_sms;
   float sm_scale;
-  float *ws;  // sched_attn_scored_ws_floats() floats
+  float *ws;  // sched_attn_scored_ws_floats() floats (none for the one-kernel form)
   long long ws_floats;
   int *status;
 };

@@ -274,6 +274,32 @@ def test_scored_many_requests():
     run_scored([37 + 13 * (i % 11) for i in range(200)], 1, 8, 8, 64, BF)
 
 
+@pytest.mark.parametrize("n,Hq,Hkv,D", [(8192, 8, 2, 128), (8100, 16, 1, 64), (4097, 16, 1, 128), (1025, 3, 1, 64)])
+def test_scored_one_kernel_form(n, Hq, Hkv, D):
+    """Few heads: one kernel, up to its longest contexts, and the two-kernel
+    form of the same call among many more requests."""
+    from sched_pass_b200 import _ext
+    lens = [n, 1, 0, n // 3]
+    n0 = _ext.launches()
+    run_scored(lens, 1, Hq, Hkv, D, BF, seed=n)
+    assert _ext.launches() - n0 == 1
+    q, kc, vc, bt, kl, scores0 = scored_inputs(lens, 1, Hq, Hkv, D, BF, seed=n)
+    one, s1 = torch.empty_like(q), scores0.clone()
+    ops.attention_decode_scored(q, one, kc, vc, bt, kl, D**-0.5, s1)
+    many = 40
+    q2 = torch.cat([q, torch.zeros(many, 1, Hq, D, dtype=BF, device=DEV)])
+    bt2 = torch.cat([bt, torch.zeros(many, bt.shape[1], dtype=torch.int32, device=DEV)])
+    two, s2 = torch.empty_like(q2), scores0.clone()
+    n0 = _ext.launches()
+    ops.attention_decode_scored(q2, two, kc, vc, bt2, torch.cat([kl, torch.zeros(many, dtype=torch.int32, device=DEV)]),
+                                D**-0.5, s2)
+    assert _ext.launches() - n0 == 2
+    assert two[4:].abs().max() == 0
+    # sums in another order: a step of the 16-bit result, 2^-18 of the weights
+    assert bool(((one.float() - two[:4].float()).abs() <= 2.0**-7 * one.float().abs() + 2.0**-10).all())
+    assert bool(((s1 - s2).abs() <= 2.0**-18 * s1).all())
+
+
 @pytest.mark.parametrize("page", [32, 48, 128])
 def test_scored_page_sizes(page):
     run_scored([0, 1, 47, 48, 49, 130, 400], 1, 8, 2, 128, BF, page=page)
@@ -450,6 +476,23 @@ def test_evict_layouts(D, dtype, page):
 def test_evict_long(n, budget):
     """Up to contexts whose keys do not fit shared memory."""
     check_evict(evict_inputs([n, n // 2], 1, 64, BF, seed=n), budget, budget // 4, 4)
+
+
+def test_evict_many_heads_and_moves():
+    """A CTA per head, with more moves than it lists at a time."""
+    check_evict(evict_inputs([5000 - 7 * i for i in range(19)], 8, 64, BF, seed=3), 2400, 100, 4)
+
+
+def test_evict_unaligned_tracking_tensors():
+    """scores and positions that do not start on a 16-byte boundary take the scalar loads."""
+    state = evict_inputs([300, 150], 2, 64, BF)
+    want = ref.kv_evict(*state, 100, 10, 2)
+    got = [t.clone() for t in state[:4]]
+    for i in (2, 3):
+        room = torch.empty(got[i].numel() + 1, dtype=got[i].dtype, device=DEV)
+        got[i] = room[1:].view(got[i].shape).copy_(state[i])
+    lens = ops.kv_evict(*got, *state[4:], 100, 10, sink=2)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(lens, want[4])
 
 
 def test_evict_more_protected_than_the_budget():
