@@ -642,7 +642,10 @@ struct RowSoftmax {
   }
 };
 
-// One warp: a run of the tile list.
+// One warp: a run of the tile list. Memory bound: 64 requests of 1536 to 1664
+// tokens (8 heads of 128, 4 query rows each) take 71 us, 92 % of the copy
+// rate, 8 of up to 32768 (8 rows) 150 us, 93 %. With 16 rows the products,
+// exponentials and logits of a tile take longer than its loads (115 us).
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kWarps * 32, resident(D, ROWS))
     scored_split_kernel(const ScoredArgs a, const ScoredPlan pl) {
@@ -774,7 +777,9 @@ __device__ __forceinline__ void add_weight(float4 &w, const float4 &s, float lse
 // cluster has a (request, KV head), its warps the tiles in turn (so that a
 // warp's first page does not depend on the length). The logits stay in shared
 // memory; the CTAs exchange (max, sum) and outputs through it, and each then
-// adds its own tokens' weights.
+// adds its own tokens' weights. Latency bound: a chain of the loads of length
+// and page, K and V, the products, two exchanges and the additions (one request
+// of 700 tokens: 6.4 us).
 constexpr int kCluster = 8;   // CTAs
 constexpr int kCWarps = 8;    // warps of each
 constexpr int kCTiles = 8;    // tiles of a warp at most (8192 tokens)
@@ -1082,6 +1087,11 @@ __host__ __device__ __forceinline__ size_t evict_words(int n) { return (size_t)(
 // slot. A flag marks the slots below the budget that lose their token and the
 // slots behind it that keep theirs; as many of the one as of the other, so one
 // prefix sum over the flags ranks both.
+//
+// Measured: 64 requests of 2112 slots to 2048, 8 heads of 128: 19 us, of which
+// reading scores and positions would take 3: the rest is the issue and the
+// barriers of the selection. 16 of 8192 to 2048: 52 us, 14 of selection and
+// then 206 MB of moves at the copy rate.
 template <int D, bool IN_WS>
 __global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32_t *ws, int vec, int page_shift) {
   extern __shared__ __align__(16) uint32_t dyn[];  // evict_words(max_len) unless they are in the workspace (IN_WS)
