@@ -919,6 +919,7 @@ void kv_evict(at::Tensor &k_cache, at::Tensor &v_cache, at::Tensor &scores, at::
   const int64_t ps = k_cache.size(2);
   check_track(scores, k_cache, at::kFloat, "scores", "float32");
   check_track(positions, k_cache, at::kInt, "positions", "int32");
+  TORCH_CHECK(scores.numel() < 0xffffffffll, "the cache must have fewer than 2^32 - 1 rows");
   TORCH_CHECK(kv_lens.dim() == 1, "kv_lens must be [requests]");
   const int64_t R = kv_lens.size(0);
   check_vec(kv_lens, at::kInt, R, "kv_lens", "int32");

@@ -386,10 +386,12 @@ __device__ __forceinline__ void mma16816<__half>(float &d0, float &d1, float &d2
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// read once: not kept in L1, and the first to leave L2 (which the logits should not)
+// Read once: not kept in L1, and the first to leave L2 (which the logits should
+// not). Not the read-only path: the kernel in front may still write the cache
+// when this one starts (programmatic dependent launch).
 __device__ __forceinline__ uint4 ld_stream(const void *p, uint64_t policy) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
+  asm volatile("ld.global.L1::no_allocate.L2::cache_hint.v4.u32 {%0,%1,%2,%3}, [%4], %5;"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p), "l"(policy));
   return v;
@@ -794,7 +796,7 @@ __global__ void __launch_bounds__(kCWarps * 32) scored_cluster_kernel(const Scor
   float *o_w = sm;                            // [kCWarps][ROWS][D]; the first [ROWS][D] then hold the CTA's
   float *s_sm = sm + kCWarps * ROWS * D;      // [rows][span]
   const int rank = (int)ptx::cluster_ctarank();
-  const int req = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int req = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, warp = tid / 32;
   const int G = a.Hq / a.Hkv;
   ptx::pdl_launch_dependents();
   ptx::pdl_wait();

@@ -260,8 +260,8 @@ def attention_decode_scored(q: torch.Tensor, out: torch.Tensor, k_cache: torch.T
     whose weights start its tokens' scores. A row that sees nothing gives zeros
     and lse = -inf. ``lse`` float32 of q's shape without D: natural log of the
     softmax's sum. ``max_len``: a bound of the kv_lens that the host knows
-    (0: the block table's width); it sizes the scratch, and a longer length is
-    reported and cut. bf16 or fp16, D 64 or 128, page size a multiple of 16,
+    (0: the block table's width); it sizes the scratch (4 bytes per request,
+    query, query head and token), and a longer length is reported and cut. bf16 or fp16, D 64 or 128, page size a multiple of 16,
     any Hq / Hkv.
 
     The pages of one call's requests should be distinct: in a page that two
@@ -289,8 +289,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     Returns the new lengths, int32 [R] = min(kv_lens, budget): further tokens
     are appended from there, and the pages behind are free. The cache is not
     read where a request fits its budget. ``max_len`` as in
-    ``attention_decode_scored``. Pages must not be shared by requests (nor with
-    a prefix cache). Pages outside the cache are reported; their tokens go
+    ``attention_decode_scored``. A page must not be named twice: not by two
+    requests (nor a prefix cache) and not within one. Pages outside the cache are reported; their tokens go
     first and are not moved."""
     if new_lens is None:
         new_lens = torch.empty_like(kv_lens)

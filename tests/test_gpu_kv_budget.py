@@ -700,6 +700,18 @@ def test_long_cache_offsets_pass_32_bits():
         assert torch.equal(a[last], b)
 
 
+def test_scratch_that_does_not_fit_is_an_error_of_the_call():
+    """A table of 2^29 tokens without max_len asks for 275 GB of logits."""
+    k = torch.zeros(2, 8, 16, 64, dtype=BF, device=DEV)
+    bt = torch.zeros(1, 1 << 25, dtype=torch.int32, device=DEV)
+    q = torch.ones(1, 128, 64, dtype=BF, device=DEV)
+    sc = torch.zeros(2, 8, 16, device=DEV)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.attention_decode_scored(q, torch.empty_like(q), k, k, bt, i32([20]), 1.0, sc)
+    out = ops.attention_decode_scored(q, torch.empty_like(q), k, k, bt, i32([20]), 1.0, sc, max_len=32)
+    assert out.abs().max() == 0 and (sc[0, :, :4].sum() > 0)
+
+
 def test_calls_without_work():
     k = torch.zeros(2, 2, 16, 64, dtype=BF, device=DEV)
     sc, ps = torch.zeros(2, 2, 16, device=DEV), torch.zeros(2, 2, 16, dtype=torch.int32, device=DEV)
