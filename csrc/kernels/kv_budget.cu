@@ -356,7 +356,8 @@ inline ScoredPlan scored_plan(int R, int Q, int Hq, int Hkv, int D, int max_len,
   while (heads * ((max_len + p.join - 1) / p.join) > 4ll * num_sms && p.join < max_len) p.join += p.join < 1024 ? p.join : 1024;
   // and at most 16 partial results per warp
   p.o_rows = 1;
-  while (p.o_rows < 8 && heads * ((p.rows + p.o_rows - 1) / p.o_rows) > num_sms && p.grid * kWarps / tasks * p.o_rows * 2 <= 8 * 16)
+  while (p.o_rows < 32 && heads * ((p.rows + p.o_rows - 1) / p.o_rows) > (p.o_rows < 8 ? 1 : 4) * num_sms &&
+         p.grid * kWarps / tasks * p.o_rows * 2 <= 8 * 16)
     p.o_rows *= 2;
   p.s_off = 0;
   p.o_off = heads * p.rows * p.lp;
@@ -642,6 +643,37 @@ struct RowSoftmax {
       }
     }
   }
+  // The same where these were all of the task's tiles: its outputs and lse.
+  __device__ __forceinline__ void finish_task(const ScoredArgs &a, int req, int h, int row0, float2 *ml_out) {
+    const int G = a.Hq / a.Hkv;
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+      const int row = r + 8 * i;
+      if (row < rows_here) {
+        const bool none = m[i] == -INFINITY && sum[i] == 0.f;  // a row that sees nothing
+        const float f = none ? 0.f : 1.f / sum[i];
+        const int qi = (row0 + row) / G, g = row0 + row - qi * G;
+        T *dst = static_cast<T *>(a.out) + (size_t)req * a.out_req + (size_t)qi * a.out_query + (size_t)(h * G + g) * D + 16 * c;
+#pragma unroll
+        for (int d = 0; d < D / 64; ++d)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float v[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = o[d * 8 + x][2 * i + e] * f;
+            *reinterpret_cast<uint4 *>(dst + d * 64 + 8 * e) =
+                make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+          }
+        if (c == 0) {
+          ml_out[row] = make_float2(m[i], sum[i]);
+          if (a.lse != nullptr)
+            a.lse[((size_t)req * a.Q + qi) * a.Hq + h * G + g] = none ? -INFINITY : (m[i] + log2f(sum[i])) * kLn2;
+        }
+      }
+    }
+  }
 };
 
 // One warp: a run of the tile list. Memory bound: 64 requests of 1536 to 1664
@@ -720,10 +752,13 @@ __global__ void __launch_bounds__(kWarps * 32, resident(D, ROWS))
     const int h = hb / pl.blocks, row0 = (hb - h * pl.blocks) * ROWS, nt = tiles_of(n);
     x.enter(a, pl.rows, req, h, row0, n, q_sm[warp]);
     float *s_out = a.ws + pl.s_off + (((size_t)req * a.Hkv + h) * pl.rows + row0) * pl.lp;
+    const bool from_start = tile == 0;
+    bool to_end;
     int n_req = req, n_hb = hb, n_n = n;
     while (true) {  // a tile
       --left;
-      const bool ends = tile + 1 == nt || left == 0;
+      to_end = tile + 1 == nt;
+      const bool ends = to_end || left == 0;
       int n_tile = tile + 1;
       long long next = -1;
       if (left > 0) {
@@ -745,7 +780,13 @@ __global__ void __launch_bounds__(kWarps * 32, resident(D, ROWS))
       if (ends) break;
     }
     const size_t part = (size_t)w_id + (uint32_t)req * HB + hb;
-    x.finish(a.ws + pl.o_off + part * ROWS * D, reinterpret_cast<float2 *>(a.ws + pl.ml_off) + part * ROWS);
+    float2 *ml_out = reinterpret_cast<float2 *>(a.ws + pl.ml_off) + part * ROWS;
+    // whole tasks end here with 16 rows (windows of short contexts have many;
+    // with 8 rows there are few, and the code costs the loop registers)
+    if (ROWS == 16 && from_start && to_end)
+      x.finish_task(a, req, h, row0, ml_out);
+    else
+      x.finish(a.ws + pl.o_off + part * ROWS * D, ml_out);
     if (left == 0) return;
     req = n_req, hb = n_hb, n = n_n;
   }
@@ -775,33 +816,34 @@ __device__ __forceinline__ void add_weight(float4 &w, const float4 &s, float lse
   w.w += ex2_approx(s.w - lse2);
 }
 
-// The same in one kernel, for few and short contexts, where latency counts: a
-// cluster has a (request, KV head), its warps the tiles in turn (so that a
-// warp's first page does not depend on the length). The logits stay in shared
-// memory; the CTAs exchange (max, sum) and outputs through it, and each then
-// adds its own tokens' weights. Latency bound: a chain of the loads of length
-// and page, K and V, the products, two exchanges and the additions (one request
-// of 700 tokens: 6.4 us).
-constexpr int kCluster = 8;   // CTAs
-constexpr int kCWarps = 8;    // warps of each
-constexpr int kCTiles = 8;    // tiles of a warp at most (8192 tokens)
+// The same in one kernel, where latency counts: a cluster of C CTAs has a
+// (request, KV head), its warps the tiles in turn (so that a warp's first page
+// does not depend on the length). The logits stay in shared memory; the CTAs
+// exchange (max, sum) and outputs through it, and each then adds its own
+// tokens' weights. Eight CTAs of eight warps for few heads, four, two or one of
+// four warps for more. Latency bound: a chain of the loads of
+// length and page, K and V, the products, two exchanges and the additions (one
+// request of 700 tokens: 6.4 us).
+constexpr int kCTiles = 8;  // tiles of a warp at most
+// CTAs per SM by the registers (a third of four warps with heads of 128 costs more than it gives)
+constexpr int one_resident(int D, int warps) { return (D == 64 ? 2 : 1) * (warps == 8 ? 1 : 2); }
 
-template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kCWarps * 32) scored_cluster_kernel(const ScoredArgs a, int rows, int span) {
-  constexpr int NT = kCWarps * 32;
+template <typename T, int D, int ROWS, int C, int CW>
+__global__ void __launch_bounds__(CW * 32, one_resident(D, CW)) scored_cluster_kernel(const ScoredArgs a, int rows, int span) {
+  constexpr int NT = CW * 32;
   extern __shared__ __align__(16) float sm[];
-  __shared__ typename RowSoftmax<T, D, ROWS>::QTile q_sm[kCWarps];
-  __shared__ float2 ml_w[kCWarps][ROWS], ml_c[ROWS];
+  __shared__ typename RowSoftmax<T, D, ROWS>::QTile q_sm[CW];
+  __shared__ float2 ml_w[CW][ROWS], ml_c[ROWS];
   __shared__ float lse2[ROWS];                // +inf for a row that sees nothing
-  float *o_w = sm;                            // [kCWarps][ROWS][D]; the first [ROWS][D] then hold the CTA's
-  float *s_sm = sm + kCWarps * ROWS * D;      // [rows][span]
-  const int rank = (int)ptx::cluster_ctarank();
+  float *o_w = sm;                            // [CW][ROWS][D]; the first [ROWS][D] then hold the CTA's
+  float *s_sm = sm + CW * ROWS * D;      // [rows][span]
+  const int rank = C > 1 ? (int)ptx::cluster_ctarank() : 0;
   const int req = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, warp = tid / 32;
   const int G = a.Hq / a.Hkv;
   ptx::pdl_launch_dependents();
   ptx::pdl_wait();
   const int cap = table_cap(a.max_len, a.bt_pages, a.page_size);
-  int tile = rank + kCluster * warp;
+  int tile = rank + C * warp;
   const int page0 = tile * kTile < cap ? a.block_table[(size_t)req * a.bt_stride + tile * kTile / a.page_size] : -1;
   const int n = checked_len(a.kv_lens[req], cap, a.status, kSiteScoredLen, h == 0 && rank == 0 && tid == 0);
   const int nt = (n + kTile - 1) / kTile;
@@ -814,8 +856,8 @@ __global__ void __launch_bounds__(kCWarps * 32) scored_cluster_kernel(const Scor
   }
   x.enter(a, rows, req, h, 0, n, q_sm[warp]);
   const float scale2 = a.sm_scale * kLog2e;
-  for (int at = warp * kTile; tile < nt; at += kCWarps * kTile) {
-    const int n_tile = tile + kCluster * kCWarps;
+  for (int at = warp * kTile; tile < nt; at += CW * kTile) {
+    const int n_tile = tile + C * CW;
     const long long next = n_tile < nt ? tile_base(a, req, h, n_tile * kTile) : -1;
     x.step(a, base, tile * kTile, n, scale2, q_sm[warp], s_sm + at, span, n_tile < nt, next);
     tile = n_tile;
@@ -828,9 +870,9 @@ __global__ void __launch_bounds__(kCWarps * 32) scored_cluster_kernel(const Scor
     const int row = i / D;
     float top = -INFINITY, tot = 0.f, v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kCWarps; ++w) top = fmaxf(top, ml_w[w][row].x);
+    for (int w = 0; w < CW; ++w) top = fmaxf(top, ml_w[w][row].x);
 #pragma unroll
-    for (int w = 0; w < kCWarps; ++w) {
+    for (int w = 0; w < CW; ++w) {
       const float f = scale_to(ml_w[w][row].x, top);
       tot += ml_w[w][row].y * f;
       v += o_w[w * ROWS * D + i] * f;
@@ -838,24 +880,30 @@ __global__ void __launch_bounds__(kCWarps * 32) scored_cluster_kernel(const Scor
     o_w[i] = v;
     if (i % D == 0) ml_c[row] = make_float2(top, tot);
   }
-  ptx::cluster_sync_all();
+  if constexpr (C > 1)
+    ptx::cluster_sync_all();
+  else
+    __syncthreads();
   const uint32_t ml_addr = ptx::smem_u32(ml_c), o_addr = ptx::smem_u32(o_w);
   auto peer2 = [&](uint32_t addr, int cta) {
     float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(ptx::mapa_shared(addr, cta)) : "memory");
+    if constexpr (C > 1)
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(ptx::mapa_shared(addr, cta)) : "memory");
+    else
+      asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
     return v;
   };
-  {  // eight lanes to a row: a CTA's (max, sum) each
-    const int row = tid / kCluster, at = min(row, rows - 1);
-    const float2 mine = peer2(ml_addr + at * 8, tid % kCluster);
+  {  // C lanes to a row: a CTA's (max, sum) each
+    const int row = tid / C, at = min(row, rows - 1);
+    const float2 mine = peer2(ml_addr + at * 8, tid % C);
     float top = mine.x;
 #pragma unroll
-    for (int o = kCluster / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = C / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float tot = mine.y * scale_to(mine.x, top);
 #pragma unroll
-    for (int o = kCluster / 2; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
+    for (int o = C / 2; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
     const float v = top == -INFINITY && tot == 0.f ? -INFINITY : top + log2f(tot);  // NaN logits stay NaN
-    if (row < rows && tid % kCluster == 0) {
+    if (row < rows && tid % C == 0) {
       lse2[row] = v == -INFINITY ? INFINITY : v;
       if (rank == 0 && a.lse != nullptr) {
         const int qi = row / G;
@@ -865,14 +913,14 @@ __global__ void __launch_bounds__(kCWarps * 32) scored_cluster_kernel(const Scor
   }
   __syncthreads();
   // outputs: two values a thread, spread over the cluster
-  for (int i = (rank * NT + tid) * 2; i < rows * D; i += kCluster * NT * 2) {
+  for (int i = (rank * NT + tid) * 2; i < rows * D; i += C * NT * 2) {
     const int row = i / D, qi = row / G;
     const float ref = lse2[row];
-    float2 m[kCluster], p[kCluster], v = make_float2(0.f, 0.f);
+    float2 m[C], p[C], v = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < kCluster; ++k) m[k] = peer2(ml_addr + row * 8, k), p[k] = peer2(o_addr + i * 4, k);
+    for (int k = 0; k < C; ++k) m[k] = peer2(ml_addr + row * 8, k), p[k] = peer2(o_addr + i * 4, k);
 #pragma unroll
-    for (int k = 0; k < kCluster; ++k) {
+    for (int k = 0; k < C; ++k) {
       const float f = ex2_approx(m[k].x - ref);
       if (f != 0.f) v.x += p[k].x * f, v.y += p[k].y * f;
     }
@@ -880,13 +928,13 @@ __global__ void __launch_bounds__(kCWarps * 32) scored_cluster_kernel(const Scor
                                   (size_t)(h * G + row - qi * G) * D + i % D) = pack2<T>(v.x, v.y);
   }
   for (int q = tid; q < span / 4; q += NT) {  // four tokens of a tile that this CTA had
-    const int at = q * 4 / kTile, tok = ((at / kCWarps * kCWarps + at % kCWarps) * kCluster + rank) * kTile + q * 4 % kTile;
+    const int at = q * 4 / kTile, tok = ((at / CW * CW + at % CW) * C + rank) * kTile + q * 4 % kTile;
     if (tok >= n) continue;
     float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int row = 0; row < rows; ++row) add_weight(w, *reinterpret_cast<const float4 *>(s_sm + row * span + q * 4), lse2[row]);
     add_weights(a, req, h, tok, n, w);
   }
-  ptx::cluster_sync_all();  // the peers have read this CTA's shared memory
+  if constexpr (C > 1) ptx::cluster_sync_all();  // the peers have read this CTA's shared memory
 }
 
 // Join. Of a (request, KV head)'s CTAs the first ones join the outputs
@@ -944,46 +992,53 @@ __global__ void __launch_bounds__(kJoin, 4) scored_join_kernel(const ScoredArgs 
 
   if ((int)blockIdx.x < o_ctas) {
     constexpr int V = D / 32;  // values per lane
-    const int sub = kJoinWarps / pl.o_rows, row = blockIdx.x * pl.o_rows + warp / sub, part = warp % sub;
-    if (sub == 1 && row >= pl.rows) return;
-    float v[V];
+    // up to eight rows: 8 / o_rows warps to a row; more: a warp has every eighth
+    const int sub = max(1, kJoinWarps / pl.o_rows), part = warp % sub, G = a.Hq / a.Hkv;
+    const int last = min(pl.rows, (int)(blockIdx.x + 1) * pl.o_rows);
+    for (int row = blockIdx.x * pl.o_rows + warp / sub; row - warp / sub < last; row += kJoinWarps) {
+      float v[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = 0.f;
-    const int G = a.Hq / a.Hkv, qi = row / G;
-    if (row < pl.rows) {
-      const Parts pt = parts_of(before, per, nt, HB, req, h * pl.blocks + row / pl.block);
-      const float2 *mr = ml + (size_t)pt.first * pl.block + row % pl.block;
-      const float lse2 = row_lse2<32>(mr, pt.count, pl.block);
-      const float ref = lse2 == -INFINITY ? INFINITY : lse2;
-      const float *src = a.ws + pl.o_off + ((size_t)pt.first * pl.block + row % pl.block) * D + lane * V;
+      for (int e = 0; e < V; ++e) v[e] = 0.f;
+      const int qi = row / G;
+      bool done = row >= last;
+      if (!done) {
+        const Parts pt = parts_of(before, per, nt, HB, req, h * pl.blocks + row / pl.block);
+        done = pl.block == 16 && pt.count == 1;  // the warp that had all of the task has written it
+        if (!done) {
+          const float2 *mr = ml + (size_t)pt.first * pl.block + row % pl.block;
+          const float lse2 = row_lse2<32>(mr, pt.count, pl.block);
+          const float ref = lse2 == -INFINITY ? INFINITY : lse2;
+          const float *src = a.ws + pl.o_off + ((size_t)pt.first * pl.block + row % pl.block) * D + lane * V;
 #pragma unroll 4
-      for (uint32_t k = part; k < pt.count; k += sub) {
-        const float f = ex2_approx(mr[(size_t)k * pl.block].x - ref);
-        float p[V];
-        if constexpr (V == 4)
-          *reinterpret_cast<float4 *>(p) = *reinterpret_cast<const float4 *>(src + (size_t)k * pl.block * D);
-        else
-          *reinterpret_cast<float2 *>(p) = *reinterpret_cast<const float2 *>(src + (size_t)k * pl.block * D);
+          for (uint32_t k = part; k < pt.count; k += sub) {
+            const float f = ex2_approx(mr[(size_t)k * pl.block].x - ref);
+            float p[V];
+            if constexpr (V == 4)
+              *reinterpret_cast<float4 *>(p) = *reinterpret_cast<const float4 *>(src + (size_t)k * pl.block * D);
+            else
+              *reinterpret_cast<float2 *>(p) = *reinterpret_cast<const float2 *>(src + (size_t)k * pl.block * D);
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] += f != 0.f ? p[e] * f : 0.f;
+            for (int e = 0; e < V; ++e) v[e] += f != 0.f ? p[e] * f : 0.f;
+          }
+          if (part == 0 && lane == 0 && a.lse != nullptr)
+            a.lse[((size_t)req * a.Q + qi) * a.Hq + h * G + (row - qi * G)] = lse2 * kLn2;
+        }
       }
-      if (part == 0 && lane == 0 && a.lse != nullptr)
-        a.lse[((size_t)req * a.Q + qi) * a.Hq + h * G + (row - qi * G)] = lse2 * kLn2;
-    }
-    if (sub > 1) {
+      if (sub > 1) {  // (one step: o_rows < 8)
 #pragma unroll
-      for (int e = 0; e < V; ++e) sm[warp * D + lane * V + e] = v[e];
-      __syncthreads();
-      if (row >= pl.rows || part != 0) return;
-      for (int w = 1; w < sub; ++w)
+        for (int e = 0; e < V; ++e) sm[warp * D + lane * V + e] = v[e];
+        __syncthreads();
+        for (int w = 1; w < sub && part == 0; ++w)
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] += sm[(warp + w) * D + lane * V + e];
+          for (int e = 0; e < V; ++e) v[e] += sm[(warp + w) * D + lane * V + e];
+      }
+      if (done || part != 0) continue;
+      T *dst = static_cast<T *>(a.out) + (size_t)req * a.out_req + (size_t)qi * a.out_query + (size_t)(h * G + row - qi * G) * D + lane * V;
+      if constexpr (V == 4)
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+      else
+        *reinterpret_cast<uint32_t *>(dst) = pack2<T>(v[0], v[1]);
     }
-    T *dst = static_cast<T *>(a.out) + (size_t)req * a.out_req + (size_t)qi * a.out_query + (size_t)(h * G + row - qi * G) * D + lane * V;
-    if constexpr (V == 4)
-      *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
-    else
-      *reinterpret_cast<uint32_t *>(dst) = pack2<T>(v[0], v[1]);
     return;
   }
 
@@ -1390,7 +1445,8 @@ inline EvictPlan evict_plan(int R, int Hkv, int max_len, int budget, int num_sms
   // 97 us with one CTA, 29 with eight; where the heads fill the SMs a second CTA only selects once more)
   const int list = budget < max_len - budget ? budget : max_len - budget;
   p.cluster = 1;
-  while (p.cluster < 8 && list > 128 * p.cluster && heads * p.cluster * 2 * p.threads <= 1024ll * num_sms) p.cluster *= 2;
+  // (three quarters of the SMs at most: a cluster lies within a GPC)
+  while (p.cluster < 8 && list > 128 * p.cluster && heads * p.cluster * 2 * p.threads * 4 <= 3 * 1024ll * num_sms) p.cluster *= 2;
   return p;
 }
 
@@ -1433,35 +1489,72 @@ extern "C" int sched_qk_norm_rope_kv_append(const QkNormArgs *args, cudaStream_t
 }
 
 namespace kvb {
-// The one-kernel form, for a few tiles a warp and clusters that are all
-// resident at once: one CTA to an SM with heads of 128 (by its registers), two
-// with 64, and of the SMs about three quarters, since a cluster lies within a
-// GPC (14 clusters of one-to-an-SM CTAs fit, 16 do not). One request of 700
-// tokens, 8 heads of 128: 6.3 us against 9.3 with two kernels, of 8000: 19.2
-// against 20.7; 16 such heads of 1000 tokens, which do not fit: 12.5 against 11.6.
+// The one-kernel forms: where all of a call's CTAs are resident at once, with
+// as many of them per head as that allows.
 struct OneKernel {
-  int span;     // logits per row in a CTA's shared memory; 0: not this form
+  int ctas, warps;  // per (request, KV head); 0: not this form
+  int span;         // logits per row in a CTA's shared memory
   size_t smem;
 };
 inline OneKernel one_kernel(int R, int Hkv, int D, const ScoredPlan &pl, int num_sms) {
-  const int tiles = (pl.lp / kTile + kCluster * kCWarps - 1) / (kCluster * kCWarps);
-  if (pl.blocks > 1 || tiles > kCTiles) return {0, 0};
-  const int span = kCWarps * tiles * kTile;
-  const size_t smem = 4 * ((size_t)kCWarps * pl.block * D + (size_t)pl.rows * span);
-  const int resident = D == 64 && smem <= 90 * 1024 ? 2 : 1;
-  if ((long long)R * Hkv * kCluster * 4 > 3ll * num_sms * resident + 8) return {0, 0};
-  return {span, smem};
+  const OneKernel none = {0, 0, 0, 0};
+  if (pl.blocks > 1) return none;
+  auto tiles_of = [&](int ctas, int warps) { return (pl.lp / kTile + ctas * warps - 1) / (ctas * warps); };
+  auto form = [&](int ctas, int warps) {
+    const int span = warps * tiles_of(ctas, warps) * kTile;
+    return OneKernel{ctas, warps, span, 4 * ((size_t)warps * pl.block * D + (size_t)pl.rows * span)};
+  };
+  const long long heads = (long long)R * Hkv;
+  // Eight CTAs of eight warps: one to an SM with heads of 128 (by its
+  // registers), two with 64, and of the SMs about three quarters, since a
+  // cluster lies within a GPC (14 clusters of one-to-an-SM CTAs fit, 16 do
+  // not). One request of 700 tokens, 8 heads of 128: 6.4 us against 9.3 with
+  // two kernels, of 8000: 19.2 against 20.7; 16 such heads of 1000 tokens,
+  // which do not fit: 12.5 against 11.6.
+  if (tiles_of(8, 8) <= kCTiles) {
+    const OneKernel wide = form(8, 8);
+    const int per_sm = wide.smem <= 90 * 1024 ? one_resident(D, 8) : 1;  // (or by shared memory)
+    if (heads * 8 * 4 <= 3ll * num_sms * per_sm + 8) return wide;
+  }
+  // Four, two or one of four warps, with up to four tiles a warp, or eight if
+  // they fill half of the device. 8 heads of 128: 8 requests of 1000 tokens
+  // 12.2 us with four CTAs a head against 16.2 with two kernels, 16 of 500
+  // 11.7 with two against 16.4 (16.2 with four, which are not resident), 32 of
+  // 500 18.5 with one against 23.5; 4 of 2000, a quarter of the device with
+  // four of eight tiles, 17.7 against 16.5.
+  for (int c = 4; c >= 1; c /= 2) {
+    const int tiles = tiles_of(c, 4);
+    if (tiles > kCTiles) break;
+    const int per_sm = D == 64 && pl.block == 16 && tiles > 4 ? 3 : one_resident(D, 4);  // (3: shared memory)
+    const long long capacity = (long long)per_sm * num_sms;
+    if (heads * c <= capacity && (tiles <= 4 || heads * c * 2 > capacity)) return form(c, 4);
+  }
+  // More heads with contexts of a few tiles: several waves of one CTA each (64
+  // requests of 10 to 64 tokens, 8 heads of 128, 9.5 us against 14.6, of up to
+  // 250 tokens 18.7 against 19.2, of up to 500 28.1 against 25.1).
+  return tiles_of(1, 4) <= 4 ? form(1, 4) : none;
+}
+
+template <typename T, int D, int ROWS>
+auto one_kernel_for(int ctas) {
+  return ctas == 8   ? scored_cluster_kernel<T, D, ROWS, 8, 8>
+         : ctas == 4 ? scored_cluster_kernel<T, D, ROWS, 4, 4>
+         : ctas == 2 ? scored_cluster_kernel<T, D, ROWS, 2, 4>
+                     : scored_cluster_kernel<T, D, ROWS, 1, 4>;
 }
 
 template <typename T, int D>
 int run_scored(const ScoredArgs &a, const ScoredPlan &pl, cudaStream_t st) {
-  if (const OneKernel one = one_kernel(a.R, a.Hkv, D, pl, a.num_sms); one.span > 0) {
-    auto *k = pl.block == 8 ? scored_cluster_kernel<T, D, 8> : scored_cluster_kernel<T, D, 16>;
+  if (const OneKernel one = one_kernel(a.R, a.Hkv, D, pl, a.num_sms); one.ctas > 0) {
+    auto *k = pl.block == 8 ? one_kernel_for<T, D, 8>(one.ctas) : one_kernel_for<T, D, 16>(one.ctas);
     if (one.smem > 8 * 1024 &&
-        cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             4 * (kCWarps * 16 * D + 16 * kCWarps * kCTiles * kTile)) != cudaSuccess)
+        cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * one.warps * (16 * D + 16 * kCTiles * kTile)) !=
+            cudaSuccess)
       return -4;
-    return launch_cluster(k, dim3(kCluster, a.Hkv, a.R), dim3(kCWarps * 32), kCluster, one.smem, st, a, pl.rows, one.span);
+    const dim3 grid(one.ctas, a.Hkv, a.R), block(one.warps * 32);
+    if (one.ctas > 1) return launch_cluster(k, grid, block, one.ctas, one.smem, st, a, pl.rows, one.span);
+    launch_pdl(k, grid, block, one.smem, st, a, pl.rows, one.span);
+    return launched();
   }
   auto *split = pl.block == 8 ? scored_split_kernel<T, D, 8> : scored_split_kernel<T, D, 16>;
   launch_pdl(split, dim3(pl.grid), dim3(kWarps * 32), 0, st, a, pl);
@@ -1476,7 +1569,7 @@ int run_scored(const ScoredArgs &a, const ScoredPlan &pl, cudaStream_t st) {
 extern "C" long long sched_attn_scored_ws_floats(int R, int Q, int Hq, int Hkv, int D, int max_len, int num_sms) {
   if (R <= 0 || Q <= 0 || Hkv <= 0 || Hq < Hkv || max_len <= 0) return 0;
   const kvb::ScoredPlan pl = kvb::scored_plan(R, Q, Hq, Hkv, D, max_len, num_sms);
-  return kvb::one_kernel(R, Hkv, D, pl, num_sms).span > 0 ? 0 : pl.total;
+  return kvb::one_kernel(R, Hkv, D, pl, num_sms).ctas > 0 ? 0 : pl.total;
 }
 
 extern "C" int sched_attn_scored(const ScoredArgs *args, cudaStream_t st) {
@@ -1492,7 +1585,7 @@ extern "C" int sched_attn_scored(const ScoredArgs *args, cudaStream_t st) {
   const kvb::ScoredPlan pl = kvb::scored_plan(a.R, a.Q, a.Hq, a.Hkv, a.D, a.max_len, a.num_sms);
   // the tile list is indexed in 32 bits (2^31 tiles are 2^35 cached tokens and heads)
   if ((long long)a.R * a.Hkv * pl.blocks * (pl.lp / kvb::kTile) > 0x7fffffffll) return -1;
-  if (kvb::one_kernel(a.R, a.Hkv, a.D, pl, a.num_sms).span == 0 && (a.ws == nullptr || a.ws_floats < pl.total)) return -2;
+  if (kvb::one_kernel(a.R, a.Hkv, a.D, pl, a.num_sms).ctas == 0 && (a.ws == nullptr || a.ws_floats < pl.total)) return -2;
   if (a.element == kKvFp16)
     return a.D == 128 ? kvb::run_scored<__half, 128>(a, pl, st) : kvb::run_scored<__half, 64>(a, pl, st);
   return a.D == 128 ? kvb::run_scored<__nv_bfloat16, 128>(a, pl, st) : kvb::run_scored<__nv_bfloat16, 64>(a, pl, st);

@@ -300,6 +300,50 @@ def test_scored_one_kernel_form(n, Hq, Hkv, D):
     assert bool(((s1 - s2).abs() <= 2.0**-18 * s1).all())
 
 
+@pytest.mark.parametrize("R,n", [(2, 250), (9, 1000), (16, 500), (30, 500), (64, 250), (130, 100)])
+@pytest.mark.parametrize("Hq,D", [(32, 128), (128, 128), (24, 64)])
+def test_scored_one_kernel_with_fewer_ctas(R, n, Hq, D):
+    """Four, two and one CTA per head, and several waves of one."""
+    run_scored([n - (37 * i) % n for i in range(R)], 1, Hq, 8, D, BF, seed=R)
+
+
+IDLE = [0] * 300  # requests without tokens: with them a call has too many heads for the one-kernel forms
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("Q,Hq,Hkv,D", [(1, 4, 4, 64), (1, 8, 2, 128), (1, 16, 2, 128), (1, 32, 2, 64), (2, 6, 2, 128),
+                                        (3, 10, 2, 64), (20, 8, 2, 128)])
+def test_scored_two_kernel_form(Q, Hq, Hkv, D, dtype):
+    from sched_pass_b200 import _ext
+    n0 = _ext.launches()
+    run_scored([0, 1, 15, 16, 17, 300, 301, 513, 700, 1023, 64] + IDLE, Q, Hq, Hkv, D, dtype, seed=Hq)
+    assert _ext.launches() - n0 == 2
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("Q", [1, 4])
+def test_scored_two_kernels_stale_values_and_bad_pages(value, Q):
+    lens, Hq, Hkv, D = [289, 7, 300, 641] + IDLE, 8, 2, 128
+    q, kc, vc, bt, kl, scores0 = scored_inputs(lens, Q, Hq, Hkv, D, BF)
+    clean = (kc.clone(), vc.clone())
+    for r, n in enumerate(lens[:4]):
+        if n % 16:
+            kc[bt[r, n // 16], :, n % 16:] = value
+            vc[bt[r, n // 16], :, n % 16:] = value
+    scores, out, lse = scores0.clone(), torch.empty_like(q), torch.empty(q.shape[:3], device=DEV)
+    ops.attention_decode_scored(q, out, kc, vc, bt, kl, D**-0.5, scores, lse=lse)
+    check_scored(q, *clean, bt, kl, scores0, out, lse, scores, D**-0.5)
+    table = bt.clone()
+    table[2, 3], table[3, 40] = kc.shape[0], -9
+    scores = scores0.clone()
+    ops.attention_decode_scored(q, out, kc, vc, table, kl, D**-0.5, scores, lse=lse)
+    expect_bad_index(8)
+    check_scored(q, *clean, bt, kl, scores0, out, lse, scores, D**-0.5, bad=(2, 3))
+    want, z, _ = ref.attention_scored(q[:4], *clean, table, kl, D**-0.5)
+    assert (out[:4].double() - want).abs().max() < 0.02
+    assert (lse[2:4].double() - z[2:4]).abs().max() < 1e-4
+
+
 @pytest.mark.parametrize("page", [32, 48, 128])
 def test_scored_page_sizes(page):
     run_scored([0, 1, 47, 48, 49, 130, 400], 1, 8, 2, 128, BF, page=page)
