@@ -1344,8 +1344,9 @@ __global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32
     return __reduce_add_sync(0xffffffffu, lane < NW ? tot[lane] : 0u);
   };
   // Calls f(j, number of flags in front) for the flagged slots of this warp's
-  // blocks; every warp counts all blocks, 32 at a time, for itself.
-  auto flagged = [&](auto f) {
+  // blocks that wanted(first, end of their numbers) admits; every warp counts
+  // all blocks, 32 at a time, for itself.
+  auto flagged = [&](auto wanted, auto f) {
     uint32_t front = 0;
     for (int w0 = 0; w0 < nb; w0 += 32) {
       uint32_t c = 0;
@@ -1355,11 +1356,12 @@ __global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32
       }
       const uint32_t inc = warp_scan(c);
       for (int w = w0 + warp; w < min(nb, w0 + 32); w += NW) {
-        if (__shfl_sync(0xffffffffu, c, w - w0) == 0) continue;
+        const uint32_t base = front + __shfl_sync(0xffffffffu, inc - c, w - w0);
+        const uint32_t end = front + __shfl_sync(0xffffffffu, inc, w - w0);
+        if (base == end || !wanted((int)base, (int)end)) continue;
         const uint4 v = *reinterpret_cast<const uint4 *>(flags + w * 4);
         const uint32_t word[4] = {v.x, v.y, v.z, v.w}, lower = (1u << lane) - 1u;
-        uint32_t at = front + __shfl_sync(0xffffffffu, inc - c, w - w0) + __popc(v.x & lower) + __popc(v.y & lower) +
-                      __popc(v.z & lower) + __popc(v.w & lower);
+        uint32_t at = base + __popc(v.x & lower) + __popc(v.y & lower) + __popc(v.z & lower) + __popc(v.w & lower);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (word[e] >> lane & 1u) f(w * 128 + lane * 4 + e, at++);
@@ -1371,9 +1373,10 @@ __global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32
   auto bits = [](bool a, bool b, bool c, bool d) { return (uint32_t)a | (uint32_t)b << 1 | (uint32_t)c << 2 | (uint32_t)d << 3; };
   if (last_slot < 0) {
     flag([&](int, const uint4 &k) { return bits(k.x == prefix, k.y == prefix, k.z == prefix, k.w == prefix); });
-    flagged([&](int j, uint32_t at) {
-      if (at == need - 1) s_slot = j;
-    });
+    flagged([&](int base, int end) { return base < (int)need && (int)need <= end; },
+            [&](int j, uint32_t at) {
+              if (at == need - 1) s_slot = j;
+            });
     __syncthreads();
     last_slot = s_slot;
     __syncthreads();
@@ -1395,12 +1398,13 @@ __global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32
   const int share = (moves + C - 1) / C, r0 = min(moves, rank * share), r1 = min(moves, r0 + share);
   for (int q0 = r0; q0 < r1; q0 += kWindow) {
     const int cnt = min(r1 - q0, kWindow);
-    flagged([&](int j, uint32_t at) {
-      int i = (int)at - q0;
-      uint32_t *list = to;
-      if (j >= b) i -= moves, list = from;
-      if (i >= 0 && i < cnt) list[i] = (uint32_t)j;
-    });
+    flagged([&](int base, int end) { return (base < q0 + cnt && end > q0) || (base < moves + q0 + cnt && end > moves + q0); },
+            [&](int j, uint32_t at) {
+              int i = (int)at - q0;
+              uint32_t *list = to;
+              if (j >= b) i -= moves, list = from;
+              if (i >= 0 && i < cnt) list[i] = (uint32_t)j;
+            });
     __syncthreads();
     for (int i = tid; i < cnt; i += NT) {  // slots to rows, and the tracking entries
       const uint32_t src = row_of((int)from[i]);
