@@ -736,7 +736,8 @@ void check_track(const at::Tensor &t, const at::Tensor &k, at::ScalarType type, 
 }
 void check_table(const at::Tensor &bt, int64_t rows) {
   TORCH_CHECK(bt.scalar_type() == at::kInt, "block_table must be int32");
-  TORCH_CHECK(bt.dim() == 2 && bt.size(0) >= rows && bt.size(1) >= 1 && bt.stride(1) == 1 && bt.size(1) <= INT32_MAX,
+  TORCH_CHECK(bt.dim() == 2 && bt.size(0) >= rows && bt.size(1) >= 1 && (bt.stride(1) == 1 || bt.size(1) == 1) &&
+                  bt.size(1) <= INT32_MAX,
               "block_table must be [>= requests, pages per request] with contiguous rows");
 }
 void check_aligned(const at::Tensor &t, const char *name) {
@@ -775,7 +776,6 @@ void qk_norm_rope_kv_append(const at::Tensor &qkv, const at::Tensor &wq, const a
               "q_out must be [>= tokens, q heads, head dim] with contiguous heads");
   if (scores.has_value()) check_track(*scores, k_cache, at::kFloat, "scores", "float32");
   if (positions.has_value()) check_track(*positions, k_cache, at::kInt, "positions", "int32");
-  // a slot is an int32: the whole cache must be addressable by one
   TORCH_CHECK(T <= 1 || (qkv.stride(0) % 8 == 0 && q_out.stride(0) % 8 == 0 && q_out.stride(0) >= Hq * D),
               "rows of qkv and q_out must not overlap and must start on 16-byte boundaries");
   const std::pair<const at::Tensor *, const char *> on[] = {{&qkv, "qkv"}, {&wq, "q_weight"}, {&wk, "k_weight"},
@@ -911,9 +911,10 @@ int64_t attn_decode_scored(const at::Tensor &q, at::Tensor &out, const at::Tenso
   return a.ws_floats == 0 ? 1 : 2;
 }
 
-void kv_evict(at::Tensor &k_cache, at::Tensor &v_cache, at::Tensor &scores, at::Tensor &positions,
+// returns new_lens, made here unless given
+at::Tensor kv_evict(at::Tensor &k_cache, at::Tensor &v_cache, at::Tensor &scores, at::Tensor &positions,
               const at::Tensor &block_table, const at::Tensor &kv_lens, const at::Tensor &last_pos, int64_t budget,
-              int64_t recent, int64_t sink, at::Tensor &new_lens, int64_t max_len,
+              int64_t recent, int64_t sink, const c10::optional<at::Tensor> &given, int64_t max_len,
               const c10::optional<at::Tensor> &status) {
   check_cache(k_cache, v_cache);
   const int64_t ps = k_cache.size(2);
@@ -924,7 +925,7 @@ void kv_evict(at::Tensor &k_cache, at::Tensor &v_cache, at::Tensor &scores, at::
   const int64_t R = kv_lens.size(0);
   check_vec(kv_lens, at::kInt, R, "kv_lens", "int32");
   check_vec(last_pos, at::kInt, R, "last_pos", "int32");
-  check_vec(new_lens, at::kInt, R, "new_lens", "int32");
+  if (given.has_value()) check_vec(*given, at::kInt, R, "new_lens", "int32");
   check_table(block_table, R);
   TORCH_CHECK(R <= 65535, "at most 65535 requests");
   TORCH_CHECK(budget >= 1 && budget <= INT32_MAX, "budget must be at least 1");
@@ -936,10 +937,11 @@ void kv_evict(at::Tensor &k_cache, at::Tensor &v_cache, at::Tensor &scores, at::
   TORCH_CHECK(cap < (1 << 30), "contexts of 2^30 tokens or more");
   check_cuda(k_cache, "k_cache");
   const std::pair<const at::Tensor *, const char *> on[] = {{&v_cache, "v_cache"}, {&scores, "scores"},
-      {&positions, "positions"}, {&block_table, "block_table"}, {&kv_lens, "kv_lens"}, {&last_pos, "last_pos"},
-      {&new_lens, "new_lens"}};
+      {&positions, "positions"}, {&block_table, "block_table"}, {&kv_lens, "kv_lens"}, {&last_pos, "last_pos"}};
   for (const auto &t : on) check_on(*t.first, k_cache, t.second);
-  if (R == 0) return;
+  if (given.has_value()) check_on(*given, k_cache, "new_lens");
+  at::Tensor new_lens = given.has_value() ? *given : at::empty({R}, kv_lens.options());
+  if (R == 0) return new_lens;
   const int32_t *nl = new_lens.data_ptr<int32_t>(), *kl = kv_lens.data_ptr<int32_t>(), *lp = last_pos.data_ptr<int32_t>();
   TORCH_CHECK((nl + R <= kl || kl + R <= nl) && (nl + R <= lp || lp + R <= nl),
               "new_lens must not overlap kv_lens or last_pos: every head reads the old ones");
@@ -978,6 +980,7 @@ void kv_evict(at::Tensor &k_cache, at::Tensor &v_cache, at::Tensor &scores, at::
     rc_ = sched_kv_evict(&a, cur_stream());
   }
   check_rc(rc_, "kv_evict");
+  return new_lens;
 }
 
 void probe_stream(const at::Tensor &src, int64_t policy, at::Tensor &sink, int64_t grid) {

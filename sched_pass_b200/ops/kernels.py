@@ -292,11 +292,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     ``attention_decode_scored``. A page must not be named twice: not by two
     requests (nor a prefix cache) and not within one. Pages outside the cache are reported; their tokens go
     first and are not moved."""
-    if new_lens is None:
-        new_lens = torch.empty_like(kv_lens)
-    ext().kv_evict(k_cache, v_cache, scores, positions, block_table, kv_lens, last_pos, int(budget), int(recent),
-                   int(sink), new_lens, int(max_len), _status_of(k_cache))
-    return new_lens
+    return ext().kv_evict(k_cache, v_cache, scores, positions, block_table, kv_lens, last_pos, int(budget), int(recent),
+                          int(sink), new_lens, int(max_len), _status_of(k_cache))
 
 
 def attention_merge(part_o, part_lse, merge_req, merge_begin, rows, out):
