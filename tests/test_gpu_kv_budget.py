@@ -264,6 +264,20 @@ def test_scored_windows(Q, Hq, Hkv, D):
     run_scored([0, 1, 2, 3, 15, 17, 33, 64, 200], Q, Hq, Hkv, D, BF, seed=Q)
 
 
+def test_scored_most_query_rows():
+    """8192 query rows on one KV head, the most a call takes; one more is refused."""
+    run_scored([600, 37], 512, 16, 1, 64, BF)
+    q, kc, vc, bt, kl, scores = scored_inputs([40], 513, 16, 1, 64, BF)
+    with pytest.raises(RuntimeError, match="8192 query rows"):
+        ops.attention_decode_scored(q, torch.empty_like(q), kc, vc, bt, kl, 0.125, scores)
+
+
+def test_scored_thousands_of_requests():
+    lens = [0] * 3000
+    lens[5], lens[1500], lens[2999], lens[31], lens[32] = 300, 17, 1, 64, 400
+    run_scored(lens, 1, 4, 1, 64, BF)
+
+
 @pytest.mark.parametrize("n,max_len", [(700, 0), (1500, 1500), (2049, 4096), (5001, 5001)])
 def test_scored_long(n, max_len):
     run_scored([n, 1, n - 1, n // 2], 1, 8, 2, 128, BF, seed=n, max_len=max_len, cols=-(-max(n, max_len) // 16))
