@@ -324,7 +324,7 @@ struct ScoredPlan {
   int rows, lp;         // query rows per KV head, padded length
   int block, blocks;    // rows per task (8 or 16), tasks per (request, KV head)
   int grid;             // CTAs of the split kernel
-  int join, o_rows;     // tokens per weight CTA and rows per output CTA of the join
+  int join, o_rows;     // tokens per weight CTA and rows per output CTA of the join (0: no CTAs for outputs alone)
   // workspace: logits [R, Hkv, rows, lp], partial outputs and (max, sum) [parts, block],
   // and for the join: tiles per warp, then (length, tiles in front) of each request
   long long s_off, o_off, ml_off, meta_off, total;
@@ -348,6 +348,8 @@ inline ScoredPlan scored_plan(int R, int Q, int Hq, int Hkv, int D, int max_len,
   while (p.o_rows < 32 && heads * ((p.rows + p.o_rows - 1) / p.o_rows) > (p.o_rows < 8 ? 1 : 4) * num_sms &&
          p.grid * kWarps / tasks * p.o_rows * 2 <= 8 * 16)
     p.o_rows *= 2;
+  // up to eight rows and many heads: a warp of the first weight CTA has a row each
+  if (p.rows <= 8 && heads > num_sms) p.o_rows = 0;
   p.s_off = 0;
   p.o_off = heads * p.rows * p.lp;
   const long long parts = (long long)p.grid * kWarps + tasks;
@@ -966,6 +968,44 @@ __device__ __forceinline__ float row_lse2(const float2 *ml, uint32_t count, int 
   return top == -INFINITY && tot == 0.f ? -INFINITY : top + log2f(tot);
 }
 
+// This warp's share (every `sub`-th from `part`) of a row's joined output, D / 32 values a lane.
+template <int D>
+__device__ __forceinline__ void join_row(const ScoredArgs &a, const ScoredPlan &pl, const Parts &pt, int row, float lse2,
+                                         int part, int sub, float (&v)[D / 32]) {
+  constexpr int V = D / 32;
+  const size_t at = (size_t)pt.first * pl.block + row % pl.block;
+  const float2 *mr = reinterpret_cast<const float2 *>(a.ws + pl.ml_off) + at;
+  const float ref = lse2 == -INFINITY ? INFINITY : lse2;
+  const float *src = a.ws + pl.o_off + at * D + threadIdx.x % 32 * V;
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = 0.f;
+#pragma unroll 4
+  for (uint32_t k = part; k < pt.count; k += sub) {
+    const float f = ex2_approx(mr[(size_t)k * pl.block].x - ref);
+    float p[V];
+    if constexpr (V == 4)
+      *reinterpret_cast<float4 *>(p) = *reinterpret_cast<const float4 *>(src + (size_t)k * pl.block * D);
+    else
+      *reinterpret_cast<float2 *>(p) = *reinterpret_cast<const float2 *>(src + (size_t)k * pl.block * D);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] += f != 0.f ? p[e] * f : 0.f;
+  }
+}
+template <typename T, int D>
+__device__ __forceinline__ void put_row(const ScoredArgs &a, int req, int h, int row, const float (&v)[D / 32]) {
+  const int G = a.Hq / a.Hkv, qi = row / G;
+  T *dst = static_cast<T *>(a.out) + (size_t)req * a.out_req + (size_t)qi * a.out_query + (size_t)(h * G + row - qi * G) * D +
+           threadIdx.x % 32 * (D / 32);
+  if constexpr (D == 128)
+    *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+  else
+    *reinterpret_cast<uint32_t *>(dst) = pack2<T>(v[0], v[1]);
+}
+__device__ __forceinline__ void put_row_lse(const ScoredArgs &a, int req, int h, int row, float lse2) {
+  const int G = a.Hq / a.Hkv, qi = row / G;
+  if (a.lse != nullptr) a.lse[((size_t)req * a.Q + qi) * a.Hq + h * G + (row - qi * G)] = lse2 * kLn2;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoin, 4) scored_join_kernel(const ScoredArgs a, const ScoredPlan pl, int o_ctas) {
   extern __shared__ __align__(16) float sm[];
@@ -982,35 +1022,20 @@ __global__ void __launch_bounds__(kJoin, 4) scored_join_kernel(const ScoredArgs 
   if ((int)blockIdx.x < o_ctas) {
     constexpr int V = D / 32;  // values per lane
     // up to eight rows: 8 / o_rows warps to a row; more: a warp has every eighth
-    const int sub = max(1, kJoinWarps / pl.o_rows), part = warp % sub, G = a.Hq / a.Hkv;
+    const int sub = max(1, kJoinWarps / pl.o_rows), part = warp % sub;
     const int last = min(pl.rows, (int)(blockIdx.x + 1) * pl.o_rows);
     for (int row = blockIdx.x * pl.o_rows + warp / sub; row - warp / sub < last; row += kJoinWarps) {
       float v[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] = 0.f;
-      const int qi = row / G;
       bool done = row >= last;
       if (!done) {
         const Parts pt = parts_of(before, per, nt, HB, req, h * pl.blocks + row / pl.block);
         done = pl.block == 16 && pt.count == 1;  // the warp that had all of the task has written it
         if (!done) {
-          const float2 *mr = ml + (size_t)pt.first * pl.block + row % pl.block;
-          const float lse2 = row_lse2<32>(mr, pt.count, pl.block);
-          const float ref = lse2 == -INFINITY ? INFINITY : lse2;
-          const float *src = a.ws + pl.o_off + ((size_t)pt.first * pl.block + row % pl.block) * D + lane * V;
-#pragma unroll 4
-          for (uint32_t k = part; k < pt.count; k += sub) {
-            const float f = ex2_approx(mr[(size_t)k * pl.block].x - ref);
-            float p[V];
-            if constexpr (V == 4)
-              *reinterpret_cast<float4 *>(p) = *reinterpret_cast<const float4 *>(src + (size_t)k * pl.block * D);
-            else
-              *reinterpret_cast<float2 *>(p) = *reinterpret_cast<const float2 *>(src + (size_t)k * pl.block * D);
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[e] += f != 0.f ? p[e] * f : 0.f;
-          }
-          if (part == 0 && lane == 0 && a.lse != nullptr)
-            a.lse[((size_t)req * a.Q + qi) * a.Hq + h * G + (row - qi * G)] = lse2 * kLn2;
+          const float lse2 = row_lse2<32>(ml + (size_t)pt.first * pl.block + row % pl.block, pt.count, pl.block);
+          join_row<D>(a, pl, pt, row, lse2, part, sub, v);
+          if (part == 0 && lane == 0) put_row_lse(a, req, h, row, lse2);
         }
       }
       if (sub > 1) {  // (one step: o_rows < 8)
@@ -1021,18 +1046,14 @@ __global__ void __launch_bounds__(kJoin, 4) scored_join_kernel(const ScoredArgs 
 #pragma unroll
           for (int e = 0; e < V; ++e) v[e] += sm[(warp + w) * D + lane * V + e];
       }
-      if (done || part != 0) continue;
-      T *dst = static_cast<T *>(a.out) + (size_t)req * a.out_req + (size_t)qi * a.out_query + (size_t)(h * G + row - qi * G) * D + lane * V;
-      if constexpr (V == 4)
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
-      else
-        *reinterpret_cast<uint32_t *>(dst) = pack2<T>(v[0], v[1]);
+      if (!done && part == 0) put_row<T, D>(a, req, h, row, v);
     }
     return;
   }
 
   const int t0 = ((int)blockIdx.x - o_ctas) * pl.join, t1 = min(n, t0 + pl.join);
-  if (t0 >= n) return;
+  const bool both = o_ctas == 0 && t0 == 0;  // outputs too
+  if (t0 >= n && !both) return;
   constexpr int PRE = 4;
   const int quads = min(pl.join / 4, kJoin), groups = kJoin / quads, grp = tid / quads, quad = tid % quads;
   const float *s_in = a.ws + pl.s_off + ((size_t)req * a.Hkv + h) * pl.rows * pl.lp;
@@ -1052,8 +1073,14 @@ __global__ void __launch_bounds__(kJoin, 4) scored_join_kernel(const ScoredArgs 
   if (pl.rows <= kJoinWarps) {
     if (warp < pl.rows) {
       const Parts pt = parts_of(before, per, nt, HB, req, h);
-      const float v = row_lse2<32>(ml + (size_t)pt.first * pl.block + warp, pt.count, pl.block);
-      if (lane == 0) put_lse(warp, v);
+      const float lse = row_lse2<32>(ml + (size_t)pt.first * pl.block + warp, pt.count, pl.block);
+      if (lane == 0) put_lse(warp, lse);
+      if (both) {
+        float v[D / 32];
+        join_row<D>(a, pl, pt, warp, lse, 0, 1, v);
+        put_row<T, D>(a, req, h, warp, v);
+        if (lane == 0) put_row_lse(a, req, h, warp, lse);
+      }
     }
   } else {
     constexpr int LR = 8;  // lanes per row
@@ -1522,10 +1549,12 @@ inline OneKernel one_kernel(int R, int Hkv, int D, const ScoredPlan &pl, int num
     const long long capacity = (long long)per_sm * num_sms;
     if (heads * c <= capacity && (tiles <= 4 || heads * c * 2 > capacity)) return form(c, 4);
   }
-  // More heads with contexts of a few tiles: several waves of one CTA each (64
-  // requests of 10 to 64 tokens, 8 heads of 128, 9.5 us against 14.6, of up to
-  // 250 tokens 18.7 against 19.2, of up to 500 28.1 against 25.1).
-  return tiles_of(1, 4) <= 4 ? form(1, 4) : none;
+  // More heads with contexts of a few tiles: two waves of one CTA each, three
+  // with heads of 64 (64 requests of 10 to 64 tokens, 8 heads of 128, 9.5 us
+  // against 13.1 with two kernels, of up to 250 18.6 against 17.3, 128 of 64 17.8
+  // against 17.4; with heads of 64 200 of up to 250 22.7 against 28.5).
+  const long long capacity = (long long)one_resident(D, 4) * num_sms;
+  return tiles_of(1, 4) <= (D == 64 ? 4 : 2) && heads <= capacity * (D == 64 ? 3 : 2) ? form(1, 4) : none;
 }
 
 template <typename T, int D, int ROWS>
@@ -1552,7 +1581,7 @@ int run_scored(const ScoredArgs &a, const ScoredPlan &pl, cudaStream_t st) {
   auto *split = pl.block == 8 ? scored_split_kernel<T, D, 8> : scored_split_kernel<T, D, 16>;
   launch_pdl(split, dim3(pl.grid), dim3(kWarps * 32), 0, st, a, pl);
   if (cudaPeekAtLastError() != cudaSuccess) return -4;
-  const int o_ctas = (pl.rows + pl.o_rows - 1) / pl.o_rows;
+  const int o_ctas = pl.o_rows > 0 ? (pl.rows + pl.o_rows - 1) / pl.o_rows : 0;
   launch_pdl(scored_join_kernel<T, D>, dim3(o_ctas + (a.max_len + pl.join - 1) / pl.join, a.Hkv, a.R), dim3(kJoin),
              (size_t)(pl.rows + 4 * kJoin) * sizeof(float), st, a, pl, o_ctas);
   return launched();
