@@ -1462,11 +1462,13 @@ inline EvictPlan evict_plan(int R, int Hkv, int max_len, int budget, int num_sms
   p.threads = 256;
   while (p.threads < 1024 && p.threads * 9 < max_len) p.threads *= 2;
   // more CTAs per head while there are many tokens to move and SMs for them (one head of 30001 slots, 6227 moves:
-  // 97 us with one CTA, 29 with eight; where the heads fill the SMs a second CTA only selects once more)
+  // 97 us with one CTA, 27 with eight; where the heads fill the SMs a second CTA only selects once more); clusters of
+  // four and eight, which lie within a GPC, on three quarters of the SMs at most
   const int list = budget < max_len - budget ? budget : max_len - budget;
   p.cluster = 1;
-  // (three quarters of the SMs at most: a cluster lies within a GPC)
-  while (p.cluster < 8 && list > 128 * p.cluster && heads * p.cluster * 2 * p.threads * 4 <= 3 * 1024ll * num_sms) p.cluster *= 2;
+  while (p.cluster < 8 && list > 128 * p.cluster &&
+         heads * p.cluster * 2 * p.threads * 4 <= (p.cluster == 1 ? 4 : 3) * 1024ll * num_sms)
+    p.cluster *= 2;
   return p;
 }
 
