@@ -261,8 +261,8 @@ def attention_decode_scored(q: torch.Tensor, out: torch.Tensor, k_cache: torch.T
     and lse = -inf. ``lse`` float32 of q's shape without D: natural log of the
     softmax's sum. ``max_len``: a bound of the kv_lens that the host knows
     (0: the block table's width); it sizes the scratch (4 bytes per request,
-    query, query head and token), and a longer length is reported and cut. bf16 or fp16, D 64 or 128, page size a multiple of 16,
-    any Hq / Hkv.
+    query, query head and token), and a longer length is reported and cut. bf16
+    or fp16, D 64 or 128, page size a multiple of 16, any Hq / Hkv.
 
     The pages of one call's requests should be distinct: in a page that two
     requests share, both add their weights, in no fixed order. Pages outside
@@ -290,8 +290,9 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     are appended from there, and the pages behind are free. The cache is not
     read where a request fits its budget. ``max_len`` as in
     ``attention_decode_scored``. A page must not be named twice: not by two
-    requests (nor a prefix cache) and not within one. Pages outside the cache are reported; their tokens go
-    first and are not moved."""
+    requests (nor a prefix cache) and not within one. Pages outside the cache
+    are reported; their tokens go first and are not moved. ``new_lens``, if
+    given, must not overlap ``kv_lens`` or ``last_pos``."""
     return ext().kv_evict(k_cache, v_cache, scores, positions, block_table, kv_lens, last_pos, int(budget), int(recent),
                           int(sink), new_lens, int(max_len), _status_of(k_cache))
 
