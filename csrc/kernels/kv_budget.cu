@@ -15,6 +15,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kv_budget_api.h"
@@ -440,6 +441,12 @@ __device__ __forceinline__ long long tile_base(const ScoredArgs &a, int req, int
 template <typename T, int D, int ROWS>
 struct RowSoftmax {
   static constexpr int NK = D / 32, RB = ROWS / 8;
+  // The weights, at most 1, enter the product with V in the cache's type: fp16
+  // keeps its 11 bits only from 2^-14 on, and a context of many tokens behind
+  // one heavy one (whose value may be small) is made of lighter ones. So fp16
+  // weights are raised to at most 2^15, and hold all bits down to 2^-29 of the
+  // largest; o has the same factor until finish(). bf16 has fp32's range.
+  static constexpr float kRaise = std::is_same<T, __half>::value ? 32768.f : 1.f;
   typedef uint4 QTile[RB][NK][32];  // each lane reads back only what it wrote
   int lane, r, c;
   uint4 kx[2][NK], vx[D / 64][4];
@@ -544,8 +551,8 @@ struct RowSoftmax {
       }
       // the weights enter the product in the cache's type (at most half a
       // step of it each, and the sum above is of the unrounded ones)
-      pa[i][0] = pack2<T>(v[0], v[1]);
-      pa[i][1] = pack2<T>(v[2], v[3]);
+      pa[i][0] = pack2<T>(v[0] * kRaise, v[1] * kRaise);
+      pa[i][1] = pack2<T>(v[2] * kRaise, v[3] * kRaise);
     }
     if (tok + kTile > end) {  // 0 * NaN: values behind the end must not reach the product
 #pragma unroll
@@ -628,7 +635,9 @@ struct RowSoftmax {
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
             const int x = d * 8 + e % 8, y = 2 * i + e / 8;
-            *reinterpret_cast<float4 *>(dst + d * 64 + e) = make_float4(o[x][y], o[x + 1][y], o[x + 2][y], o[x + 3][y]);
+            constexpr float lower = 1.f / kRaise;
+            *reinterpret_cast<float4 *>(dst + d * 64 + e) =
+                make_float4(o[x][y] * lower, o[x + 1][y] * lower, o[x + 2][y] * lower, o[x + 3][y] * lower);
           }
         if (c == 0) ml_out[row] = make_float2(m[i], sum[i]);
       }
@@ -644,7 +653,7 @@ struct RowSoftmax {
       const int row = r + 8 * i;
       if (row < rows_here) {
         const bool none = m[i] == -INFINITY && sum[i] == 0.f;  // a row that sees nothing
-        const float f = none ? 0.f : 1.f / sum[i];
+        const float f = none ? 0.f : 1.f / kRaise / sum[i];
         const int qi = (row0 + row) / G, g = row0 + row - qi * G;
         T *dst = static_cast<T *>(a.out) + (size_t)req * a.out_req + (size_t)qi * a.out_query + (size_t)(h * G + g) * D + 16 * c;
 #pragma unroll
