@@ -1504,14 +1504,23 @@ static int launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, int c
 }
 static inline int launched() { return cudaPeekAtLastError() == cudaSuccess ? 0 : -4; }
 static inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+template <typename... P>
+static inline bool any_null(P... p) {
+  return (... || (p == nullptr));
+}
+static inline bool overlap(const int32_t *a, const int32_t *b, int n) {  // of n entries each
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b), bytes = (uintptr_t)n * sizeof(int32_t);
+  return x < y + bytes && y < x + bytes;
+}
 
 extern "C" int sched_qk_norm_rope_kv_append(const QkNormArgs *args, cudaStream_t st) {
   if (args == nullptr) return -1;
   const QkNormArgs &a = *args;
   if (a.T <= 0) return 0;
-  if (a.Hq < 1 || a.Hkv < 1 || a.page_size < 1 || a.num_pages < 1 || a.max_pos < 1) return -1;
+  if (any_null(a.qkv, a.wq, a.wk, a.pos, a.slot, a.cos_sin, a.q_out, a.k_cache, a.v_cache)) return -1;
+  if (a.Hq < 1 || a.Hkv < 1 || a.page_size < 1 || a.num_pages < 1 || a.max_pos < 1 || a.num_sms < 1) return -1;
   if ((a.D != 64 && a.D != 128) || a.rot < 16 || a.rot > a.D || a.rot % 16 != 0) return -1;
-  if (a.ld_qkv % 8 != 0 || a.ld_q % 8 != 0) return -1;
+  if (a.ld_qkv % 8 != 0 || a.ld_q % 8 != 0 || (a.T > 1 && a.ld_q < (long long)a.Hq * a.D)) return -1;
   if (!aligned16(a.qkv) || !aligned16(a.wq) || !aligned16(a.wk) || !aligned16(a.cos_sin) || !aligned16(a.q_out) ||
       !aligned16(a.k_cache) || !aligned16(a.v_cache))
     return -1;
@@ -1609,11 +1618,14 @@ extern "C" int sched_attn_scored(const ScoredArgs *args, cudaStream_t st) {
   if (args == nullptr) return -1;
   const ScoredArgs &a = *args;
   if (a.R <= 0 || a.Q <= 0) return 0;
+  if (any_null(a.q, a.out, a.k_cache, a.v_cache, a.scores, a.block_table, a.kv_lens) || a.num_sms < 1) return -1;
   if (a.Hkv < 1 || a.Hq < a.Hkv || a.Hq % a.Hkv != 0 || (a.D != 64 && a.D != 128)) return -1;
   if (a.page_size < 16 || a.page_size % 16 != 0 || a.num_pages < 1 || a.max_len < 1 || a.bt_pages < 1) return -1;
   if (a.R > 65535 || a.Hkv > 65535 || a.max_len >= 1 << 30 || (long long)a.Q * (a.Hq / a.Hkv) > 8192) return -1;
-  if (a.q_req % 8 != 0 || a.q_query % 8 != 0 || !aligned16(a.q) || !aligned16(a.k_cache) || !aligned16(a.v_cache) ||
-      !aligned16(a.scores) || !aligned16(a.ws))
+  // q, K, V and out are accessed 16 bytes at a time, as are scores and ws
+  if (a.q_req % 8 != 0 || a.q_query % 8 != 0 || a.out_req % 8 != 0 || a.out_query % 8 != 0) return -1;
+  if (!aligned16(a.q) || !aligned16(a.out) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.scores) ||
+      !aligned16(a.ws))
     return -1;
   const kvb::ScoredPlan pl = kvb::scored_plan(a.R, a.Q, a.Hq, a.Hkv, a.D, a.max_len, a.num_sms);
   // the tile list is indexed in 32 bits (2^31 tiles are 2^35 cached tokens and heads)
@@ -1634,12 +1646,16 @@ extern "C" int sched_kv_evict(const KvEvictArgs *args, cudaStream_t st) {
   if (args == nullptr) return -1;
   const KvEvictArgs &a = *args;
   if (a.R <= 0) return 0;
+  if (any_null(a.k_cache, a.v_cache, a.scores, a.positions, a.block_table, a.kv_lens, a.last_pos, a.new_lens) || a.num_sms < 1)
+    return -1;
+  if (overlap(a.new_lens, a.kv_lens, a.R) || overlap(a.new_lens, a.last_pos, a.R)) return -1;  // every head reads the old ones
   if (a.Hkv < 1 || (a.D != 64 && a.D != 128) || a.page_size < 1 || a.num_pages < 1 || a.bt_pages < 1) return -1;
   if (a.budget < 1 || a.recent < 0 || a.sink < 0 || (long long)a.recent + a.sink > a.budget || a.max_len < 1) return -1;
   if (a.R > 65535 || a.Hkv > 65535 || a.max_len >= 1 << 30 || !aligned16(a.k_cache) || !aligned16(a.v_cache)) return -1;
   if ((long long)a.num_pages * a.Hkv * a.page_size >= 0xffffffffll) return -1;  // rows are numbered in 32 bits
   const long long need = sched_kv_evict_ws_ints(a.R, a.Hkv, a.max_len, a.budget, a.num_sms);
   if (need > 0 && (a.ws == nullptr || a.ws_ints < need)) return -2;
+  if (need > 0 && !aligned16(a.ws)) return -1;  // keys and flags are read 16 bytes at a time
   const kvb::EvictPlan p = kvb::evict_plan(a.R, a.Hkv, a.max_len, a.budget, a.num_sms);
   auto *k = need > 0 ? (a.D == 128 ? kvb::evict_kernel<128, true> : kvb::evict_kernel<64, true>)
                      : (a.D == 128 ? kvb::evict_kernel<128, false> : kvb::evict_kernel<64, false>);
@@ -1648,7 +1664,7 @@ extern "C" int sched_kv_evict(const KvEvictArgs *args, cudaStream_t st) {
       cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kvb::evict_words(kvb::kKeySmem) * 4) != cudaSuccess)
     return -4;
   // vectors of four slots where pages hold whole ones
-  const int vec = a.page_size % 4 == 0 && aligned16(a.scores) && aligned16(a.positions) && aligned16(a.ws);
+  const int vec = a.page_size % 4 == 0 && aligned16(a.scores) && aligned16(a.positions);
   int shift = -1;  // log2 of the page size where it is a power of two
   if ((a.page_size & (a.page_size - 1)) == 0)
     for (shift = 0; (1 << shift) < a.page_size;) ++shift;

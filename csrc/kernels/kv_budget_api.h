@@ -1,5 +1,13 @@
 // kv_budget_api.h -- launchers of the kernels that keep a paged KV cache to a
 // budget (kv_budget.cu). Plain C structs: no torch, usable from any host.
+//
+// The launchers return 0, -1 for arguments that they refuse (nothing is
+// launched), -2 for scratch that is missing or too small, -4 where the launch
+// failed. Pointers not marked "or null" must be there; qkv, the weights,
+// cos_sin, q, out, the caches, the scores of the attention, and scratch start
+// on 16-byte boundaries, and pitches of q, out and qkv are multiples of 8
+// elements. That a pointer's memory is as large as its comment says, and on
+// the device, is the caller's part.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -23,7 +31,7 @@ struct QkNormArgs {
   float *scores;            // [num_pages, Hkv, page_size] or null: set to 0 at the new slots
   int32_t *positions;       // the same shape or null: set to the position
   int T, Hq, Hkv, D, page_size, num_pages, element, num_sms;
-  int *status;
+  int *status;  // 4 words or null
 };
 extern "C" int sched_qk_norm_rope_kv_append(const QkNormArgs *args, cudaStream_t st);
 
@@ -44,7 +52,7 @@ struct ScoredArgs {
   float sm_scale;
   float *ws;  // sched_attn_scored_ws_floats() floats (none for the one-kernel form)
   long long ws_floats;
-  int *status;
+  int *status;  // 4 words or null
 };
 extern "C" long long sched_attn_scored_ws_floats(int R, int Q, int Hq, int Hkv, int D, int max_len, int num_sms);
 extern "C" int sched_attn_scored(const ScoredArgs *args, cudaStream_t st);
@@ -58,11 +66,11 @@ struct KvEvictArgs {
   long long bt_stride;
   int bt_pages;
   const int32_t *kv_lens, *last_pos;  // [R]
-  int32_t *new_lens;                  // [R]
+  int32_t *new_lens;                  // [R], apart from kv_lens and last_pos
   int R, Hkv, D, page_size, num_pages, max_len, budget, recent, sink, num_sms;
   int32_t *ws;  // sched_kv_evict_ws_ints() words
   long long ws_ints;
-  int *status;
+  int *status;  // 4 words or null
 };
 extern "C" long long sched_kv_evict_ws_ints(int R, int Hkv, int max_len, int budget, int num_sms);
 extern "C" int sched_kv_evict(const KvEvictArgs *args, cudaStream_t st);
