@@ -697,6 +697,32 @@ void moe_combine_norm(int64_t c, int64_t K, at::Tensor &h, const at::Tensor &w, 
   check_rc(rc_, "moe_combine_norm");
 }
 
+// The status words of a device (int32 x 4, zero), for the life of the process,
+// with a CUDA error code (thrown by the caller: see check_rc). They come from
+// the driver and not from torch's allocator, and are zeroed before this
+// returns, on a stream of their own: so a first use inside a graph capture
+// puts neither the memory nor the zero fill into the graph, whose replays
+// would erase reports, and a first use on one stream is in order for all.
+std::tuple<int64_t, c10::optional<at::Tensor>> status_words(int64_t device) {
+  int32_t *p = nullptr;
+  cudaError_t rc = cudaSuccess;
+  {
+    c10::cuda::CUDAGuard g((c10::DeviceIndex)device);
+    cudaStream_t st = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // of this thread: a capture elsewhere takes no part
+    if (rc = cudaThreadExchangeStreamCaptureMode(&mode); rc == cudaSuccess) {
+      rc = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+      if (rc == cudaSuccess) rc = cudaMalloc(reinterpret_cast<void **>(&p), 4 * sizeof(int32_t));
+      if (rc == cudaSuccess) rc = cudaMemsetAsync(p, 0, 4 * sizeof(int32_t), st);
+      if (rc == cudaSuccess) rc = cudaStreamSynchronize(st);
+      if (st != nullptr) cudaStreamDestroy(st);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+  }
+  if (rc != cudaSuccess) return {(int64_t)rc, c10::nullopt};
+  return {0, at::from_blob(p, {4}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)device))};
+}
+
 // ---------------------------------------------------------------- KV budget (kv_budget_api.h)
 // Shapes and types are checked before devices, so that a wrong call is refused
 // the same way on a machine without a GPU.
@@ -1148,6 +1174,7 @@ void register_symm(py::module &m);
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_symm(m);
   m.def("take_error", &take_error);
+  m.def("status_words", &status_words);
   m.def("gemm_allreduce", &gemm_allreduce);
   m.def("gemm_reduce_scatter", &gemm_reduce_scatter);
   m.def("sp_reduce_norm", &sp_reduce_norm);

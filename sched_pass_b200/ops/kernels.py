@@ -16,13 +16,18 @@ _ws: dict[tuple[int, int], "Workspace"] = {}
 def status_buffer(device=None) -> torch.Tensor:
     """The kernels' status words (int32 x 4): [0] a KernelStatus code, set by
     the first bounded wait that gives up or the first out-of-range index
-    (0 = OK); for a bad index [1] names the site and [2..3] hold the index."""
+    (0 = OK); for a bad index [1] names the site and [2..3] hold the index.
+    One buffer per device for the life of the process, in order for every
+    stream and outside any graph, whatever the first call that needs it."""
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     with _lock:
         t = _status.get(idx)
         if t is None:
-            t = torch.zeros(4, dtype=torch.int32, device=f"cuda:{idx}")
+            torch.cuda.init()
+            rc, t = ext().status_words(idx)
+            if rc:
+                raise RuntimeError(f"status words of cuda:{idx}: CUDA error {rc}")
             _status[idx] = t
     return t
 

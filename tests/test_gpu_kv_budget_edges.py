@@ -9,7 +9,7 @@ import torch
 
 from sched_pass_b200 import _ext, ops
 from sched_pass_b200.models import reference as ref
-from test_gpu_kv_budget import BF, DEV, FP, gen, i32, paged
+from test_gpu_kv_budget import BF, DEV, FP, expect_bad_index, gen, i32, paged, randn, rope_table
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,68 @@ def test_scored_many_light_tokens_behind_a_heavy_one(lens, Q, Hq, Hkv, D, launch
     err = (out.double() - want).abs()
     assert bool((err <= tol).all()), (err / tol).max()
     assert bool(((lse.double() - z).abs() <= gap * 2.0**-21 + 2.0**-20 + (n + 8) * 2.0**-24).all())
+
+
+# ------------------------------------------------------------------ the status words
+def test_status_words_made_in_a_capture_outlive_replays(monkeypatch):
+    """The first call that needs the status words is being captured: a replay
+    neither erases what another call reported nor owns the words."""
+    from sched_pass_b200.ops import kernels
+    Hq, Hkv, D = 4, 2, 64
+    g = gen(0)
+    kc, vc = randn(g, 3, Hkv, 16, D, dtype=BF), randn(g, 3, Hkv, 16, D, dtype=BF)
+    q, scores, bt, lens = randn(g, 1, Hq, D, dtype=BF), torch.zeros(3, Hkv, 16, device=DEV), i32([[2, 0]]), i32([20])
+    out = torch.empty_like(q)
+    qkv, w, cs = randn(g, 1, (Hq + 2 * Hkv) * D, dtype=BF), torch.ones(D, dtype=BF, device=DEV), rope_table(4, D)
+
+    def attend():
+        ops.attention_decode_scored(q, out, kc, vc, bt, lens, 0.1, scores)
+
+    def append(slot):
+        ops.qk_norm_rope_kv_append(qkv, w, w, 1e-5, i32([1]), slot, cs, q, kc, vc, Hq, Hkv)
+
+    attend()  # lazy loading, before any capture
+    append(i32([-1]))
+    torch.cuda.synchronize()
+    monkeypatch.setattr(kernels, "_status", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend()
+    words = ops.status_buffer()
+    assert words.tolist() == [0, 0, 0, 0]
+    graph.replay()
+    ops.check_status()
+    append(i32([3 * 16 + 5]))  # a slot behind the cache
+    graph.replay()
+    expect_bad_index(3, 53)
+    bt[0, 1] = -4
+    graph.replay()
+    expect_bad_index(8, -4)
+    bt[0, 1] = 0
+    append(i32([3 * 16 + 6]))
+    torch.cuda.synchronize()
+    del graph
+    junk = [torch.full((4,), 7, dtype=torch.int32, device=DEV) for _ in range(64)]  # whoever takes over the graph's memory
+    assert ops.status_buffer() is words and junk
+    expect_bad_index(3, 54)
+
+
+def test_status_words_of_another_stream_are_in_order(monkeypatch):
+    """Made while their stream has work queued, used at once on another."""
+    from sched_pass_b200.ops import kernels
+    Hq, Hkv, D = 4, 2, 64
+    kc = torch.zeros(3, Hkv, 16, D, dtype=BF, device=DEV)
+    vc, q = torch.zeros_like(kc), torch.zeros(1, Hq, D, dtype=BF, device=DEV)
+    qkv, w, cs = torch.ones(1, (Hq + 2 * Hkv) * D, dtype=BF, device=DEV), torch.ones(D, dtype=BF, device=DEV), rope_table(4, D)
+    pos, slot = i32([1]), i32([48])
+    big = torch.zeros(1 << 28, device=DEV)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    monkeypatch.setattr(kernels, "_status", {})
+    for _ in range(20):
+        big.add_(1)
+    ops.status_buffer()
+    with torch.cuda.stream(side):
+        ops.qk_norm_rope_kv_append(qkv, w, w, 1e-5, pos, slot, cs, q, kc, vc, Hq, Hkv)
+    torch.cuda.synchronize()
+    expect_bad_index(3, 48)
