@@ -174,7 +174,8 @@ def linear_qkv_rope(x, w, pos, slot, cos_sin, q_out, k_cache, v_cache, n_q_heads
                     grid: int = 0, ws: Workspace | None = None, x_ready: int = 0):
     """Fused QKV projection + RoPE + KV append: q heads rotated into q_out,
     k heads rotated and v heads copied into their paged-cache slots.
-    ``x_ready`` as in ``linear``."""
+    ``x_ready`` as in ``linear``. Does not start a slot's tracking (see
+    ``kv_evict``)."""
     ws = _ws_for(x, w.shape[0], x.shape[1], grid, ws)
     ext().gemm_qkv_rope(x, w, pos, slot, cos_sin, q_out, k_cache, v_cache, int(n_q_heads),
                         int(n_kv_heads), int(grid), ws.ws, ws.counters, status_buffer(x.device),
@@ -194,6 +195,9 @@ def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Te
 def rope_kv_append(qkv: torch.Tensor, pos: torch.Tensor, slot: torch.Tensor, cos_sin: torch.Tensor,
                    q_out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                    n_q_heads: int, n_kv_heads: int) -> torch.Tensor:
+    """RoPE of the query heads into q_out and of the key heads into their paged
+    slots, value heads copied; ``slot`` < 0 writes no cache entry. Does not
+    start a slot's tracking (see ``kv_evict``)."""
     ext().rope_kv_append(qkv, pos, slot, cos_sin, q_out, k_cache, v_cache, n_q_heads, n_kv_heads,
                          status_buffer(qkv.device))
     return q_out
@@ -292,8 +296,20 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     The order of the slots is then no longer that of the positions (attention
     does not need it: keys carry their rotation; ``positions`` keeps track).
     Returns the new lengths, int32 [R] = min(kv_lens, budget): further tokens
-    are appended from there, and the pages behind are free. The cache is not
-    read where a request fits its budget. ``max_len`` as in
+    are appended from there, and the pages behind are free.
+
+    Whoever appends to a slot starts its tracking, or the new token has the
+    weight and the position of the one that was there: ``qk_norm_rope_kv_append``
+    does it when it is given ``scores`` and ``positions``; ``rope_kv_append`` and
+    ``linear_qkv_rope`` do not, and after them (for tokens with slot >= 0)
+
+        scores[slot // page_size, :, slot % page_size] = 0
+        positions[slot // page_size, :, slot % page_size] = pos[:, None]
+
+    A token's slot follows from its request's length, not from its position:
+    after an eviction the two differ.
+
+    The cache is not read where a request fits its budget. ``max_len`` as in
     ``attention_decode_scored``. A page must not be named twice: not by two
     requests (nor a prefix cache) and not within one. Pages outside the cache
     are reported; their tokens go first and are not moved. ``new_lens``, if

@@ -119,3 +119,37 @@ def test_status_words_of_another_stream_are_in_order(monkeypatch):
         ops.qk_norm_rope_kv_append(qkv, w, w, 1e-5, pos, slot, cs, q, kc, vc, Hq, Hkv)
     torch.cuda.synchronize()
     expect_bad_index(3, 48)
+
+
+# ------------------------------------------------------------------ slots that an eviction freed
+def test_evict_after_appends_that_start_no_tracking():
+    """Tokens appended to freed slots by rope_kv_append: with the two
+    assignments that kv_evict documents they are new tokens to the next
+    eviction, and their entries are the old tokens' until then."""
+    Hq, Hkv, D, budget, n = 4, 2, 128, 40, 64
+    g = gen(8)
+    bt, P = paged([n, n], 16)
+    kc, vc, scores = randn(g, P, Hkv, 16, D, dtype=BF), randn(g, P, Hkv, 16, D, dtype=BF), torch.rand(P, Hkv, 16, generator=g, device=DEV)
+    positions = torch.full((P, Hkv, 16), -1, dtype=torch.int32, device=DEV)
+    positions[bt.long()] = torch.arange(n, dtype=torch.int32, device=DEV).view(1, 4, 1, 16).expand(2, 4, Hkv, 16)
+    lens = ops.kv_evict(kc, vc, scores, positions, bt, i32([n, n]), i32([n - 1, n - 1]), budget, 8, sink=2)
+    assert lens.tolist() == [budget] * 2
+    cs, q = rope_table(n + 12, D), torch.empty(2, Hq, D, dtype=BF, device=DEV)
+    for step in range(10):
+        pos = i32([n + step] * 2)
+        slot = bt[:, int(lens[0]) // 16] * 16 + lens % 16
+        page, off = (slot // 16).long(), (slot % 16).long()
+        stale = scores[page, :, off].clone(), positions[page, :, off].clone()
+        ops.rope_kv_append(randn(g, 2, (Hq + 2 * Hkv) * D, dtype=BF), pos, slot, cs, q, kc, vc, Hq, Hkv)
+        assert torch.equal(scores[page, :, off], stale[0]) and torch.equal(positions[page, :, off], stale[1])
+        scores[slot // 16, :, slot % 16] = 0
+        positions[slot // 16, :, slot % 16] = pos[:, None]
+        lens = lens + 1
+    state = [kc, vc, scores, positions]
+    want = ref.kv_evict(*state, bt, lens, i32([n + 9] * 2), budget, 8, 2)
+    got = ops.kv_evict(*state, bt, lens, i32([n + 9] * 2), budget, 8, sink=2)
+    assert all(torch.equal(a, b) for a, b in zip((*state, got), want))
+    for r in range(2):
+        for h in range(Hkv):
+            kept = positions[bt[r].long(), h].reshape(-1)[:budget].tolist()
+            assert len(set(kept)) == budget and set(range(n + 2, n + 10)) | {0, 1} <= set(kept)
