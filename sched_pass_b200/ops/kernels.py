@@ -266,12 +266,13 @@ def attention_decode_scored(q: torch.Tensor, out: torch.Tensor, k_cache: torch.T
     q and out [R, Hq, D] (one new token per request) or [R, Q, Hq, D]: the last
     Q tokens of each request, each seeing itself and what is before it (query i
     sees the first kv_lens[r] - (Q - 1 - i) tokens), e.g. the end of a prompt,
-    whose weights start its tokens' scores. A row that sees nothing gives zeros
-    and lse = -inf. ``lse`` float32 of q's shape without D: natural log of the
-    softmax's sum. ``max_len``: a bound of the kv_lens that the host knows
-    (0: the block table's width); it sizes the scratch (4 bytes per request,
-    query, query head and token), and a longer length is reported and cut. bf16
-    or fp16, D 64 or 128, page size a multiple of 16, any Hq / Hkv.
+    whose weights start its tokens' scores. A row that sees nothing, or nothing
+    but logits of -inf, gives zeros and lse = -inf. ``lse`` float32 of q's shape
+    without D: natural log of the softmax's sum. ``max_len``: a bound of the
+    kv_lens that the host knows (0: the block table's width); it sizes the
+    scratch (4 bytes per request, query, query head and token), and a longer
+    length is reported and cut. bf16 or fp16, D 64 or 128, page size a multiple
+    of 16, any Hq / Hkv.
 
     The pages of one call's requests should be distinct: in a page that two
     requests share, both add their weights, in no fixed order. Pages outside

@@ -153,3 +153,16 @@ def test_evict_after_appends_that_start_no_tracking():
         for h in range(Hkv):
             kept = positions[bt[r].long(), h].reshape(-1)[:budget].tolist()
             assert len(set(kept)) == budget and set(range(n + 2, n + 10)) | {0, 1} <= set(kept)
+
+
+def test_scored_row_of_logits_that_are_all_minus_infinity():
+    for lens in ([40, 17], [40, 17] + [0] * 300):  # one kernel, two kernels
+        bt, P = paged(lens, 16)
+        kc = torch.zeros(P, 2, 16, 64, dtype=BF, device=DEV)
+        kc[..., 0] = -float("inf")
+        vc, q = torch.ones_like(kc), torch.zeros(len(lens), 4, 64, dtype=BF, device=DEV)
+        q[..., 0] = 1
+        q[..., 1] = 1
+        out, lse, scores = torch.full_like(q, 3.0), torch.zeros(len(lens), 4, device=DEV), torch.full((P, 2, 16), 0.5, device=DEV)
+        ops.attention_decode_scored(q, out, kc, vc, bt, i32(lens), 1.0, scores, lse=lse)
+        assert out.abs().max() == 0 and bool((lse == -float("inf")).all()) and bool((scores == 0.5).all())
