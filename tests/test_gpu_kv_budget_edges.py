@@ -9,7 +9,8 @@ import torch
 
 from sched_pass_b200 import _ext, ops
 from sched_pass_b200.models import reference as ref
-from test_gpu_kv_budget import BF, DEV, FP, expect_bad_index, gen, i32, paged, randn, rope_table
+from test_gpu_kv_budget import (BF, DEV, FP, Budget, evict_inputs, expect_bad_index, gen, i32, paged, randn, rope_table,
+                                run_scored, scored_inputs)
 
 pytestmark = pytest.mark.gpu
 
@@ -166,3 +167,150 @@ def test_scored_row_of_logits_that_are_all_minus_infinity():
         out, lse, scores = torch.full_like(q, 3.0), torch.zeros(len(lens), 4, device=DEV), torch.full((P, 2, 16), 0.5, device=DEV)
         ops.attention_decode_scored(q, out, kc, vc, bt, i32(lens), 1.0, scores, lse=lse)
         assert out.abs().max() == 0 and bool((lse == -float("inf")).all()) and bool((scores == 0.5).all())
+
+
+# ------------------------------------------------------------------ the two-kernel form and its scratch
+@pytest.mark.parametrize("lens,Q,Hq,Hkv,D,dtype", [
+    ([12000], 1, 32, 8, 128, BF),                                # hundreds of partial results per row
+    ([1664 - 29 * (i % 5) for i in range(40)], 1, 32, 8, 128, BF),  # runs of many tiles over requests and heads
+    ([1500 - 31 * (i % 7) for i in range(70)], 1, 16, 4, 64, FP),
+    ([20000] + [40 + i % 9 for i in range(63)], 1, 32, 8, 128, BF),  # one long request among many short ones
+    ([9000, 3] + [17] * 98, 1, 16, 8, 64, FP),
+    ([6000, 800], 16, 8, 2, 128, BF),                            # a long window: 64 query rows
+    ([1800, 20000], 1, 64, 4, 128, FP)])                         # 16 query rows
+def test_scored_long_runs_and_uneven_batches(lens, Q, Hq, Hkv, D, dtype):
+    n0 = _ext.launches()
+    run_scored(lens, Q, Hq, Hkv, D, dtype, seed=len(lens))
+    assert _ext.launches() - n0 == 2
+
+
+@pytest.mark.parametrize("lens,Q,Hq,Hkv,D", [
+    ([1664 - 29 * (i % 5) for i in range(40)], 1, 32, 8, 128), ([900, 333, 2000], 5, 16, 2, 128), ([12000, 1], 1, 8, 8, 64)])
+def test_scored_two_kernels_repeat_bit_for_bit(lens, Q, Hq, Hkv, D):
+    q, kc, vc, bt, kl, scores0 = scored_inputs(lens, Q, Hq, Hkv, D, BF)
+    res, n0 = [], _ext.launches()
+    for i in range(5):
+        scores, out, lse = scores0.clone(), torch.empty_like(q), torch.empty(q.shape[:3], device=DEV)
+        junk = torch.full((1 << 22,), float("nan"), device=DEV)  # what the scratch holds before the call does not matter
+        del junk
+        ops.attention_decode_scored(q, out, kc, vc, bt, kl, 0.09, scores, lse=lse)
+        res.append((out, scores, lse))
+    assert _ext.launches() - n0 == 10
+    assert all(torch.equal(a, b) for x in res[1:] for a, b in zip(x, res[0]))
+
+
+def full_budget(seed, **kw):
+    """A Budget whose caches are full up to a few tokens below the budget, of
+    so many heads that the attention takes two kernels."""
+    b = Budget(seed=seed, R=300, budget=200, slack=24, **kw)
+    g = gen(seed + 100)
+    for t in (b.kc, b.vc):
+        t.copy_(randn(g, *t.shape))
+    b.scores.copy_(torch.rand(b.scores.shape, generator=g, device=DEV))
+    cols = b.bt.shape[1]
+    at = torch.arange(cols * 16, dtype=torch.int32, device=DEV).view(1, cols, 1, 16).expand(b.R, cols, b.Hkv, 16)
+    b.positions[b.bt.long()] = at
+    b.lens.copy_(190 + torch.arange(b.R, device=DEV) % 20)
+    b.pos.copy_(b.lens)
+    return b
+
+
+def same_budgets(x, y):
+    return torch.equal(x.out, y.out) and torch.equal(x.lens, y.lens) and all(torch.equal(s, t) for s, t in zip(x.state(), y.state()))
+
+
+def test_two_streams_with_scratch():
+    """As test_two_streams_at_once, where the attention needs scratch and every step evicts."""
+    pair, alone = [full_budget(s) for s in (1, 2)], [full_budget(s) for s in (1, 2)]
+    start = [x.positions.clone() for x in pair]
+    rows = randn(gen(4), 25, *pair[0].qkv.shape, dtype=BF)
+    streams = [torch.cuda.Stream() for _ in pair]
+    torch.cuda.synchronize()
+    n0 = _ext.launches()
+    for i in range(25):
+        for x, st in zip(pair, streams):
+            with torch.cuda.stream(st):
+                x.qkv.copy_(rows[i])
+                x.step()
+    assert _ext.launches() - n0 == 25 * 2 * 4  # append, two of the attention, eviction
+    torch.cuda.synchronize()
+    for i in range(25):
+        for x in alone:
+            x.qkv.copy_(rows[i])
+            x.step()
+    for x, y, p in zip(pair, alone, start):
+        assert same_budgets(x, y) and bool((x.lens == 200).all())
+        assert not torch.equal(x.positions, p)
+
+
+def test_captured_steps_with_scratch():
+    """Two graphs whose calls have scratch, replayed at once on two streams
+    with new inputs, beside eager copies."""
+    graphed, eager = [full_budget(s) for s in (5, 6)], [full_budget(s) for s in (5, 6)]
+    graphs, streams = [], [torch.cuda.Stream() for _ in graphed]
+    for x in graphed:
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        n0 = _ext.launches()
+        with torch.cuda.graph(gr):
+            x.step()
+        assert _ext.launches() - n0 == 4
+        graphs.append(gr)
+    rows = randn(gen(3), 20, *eager[0].qkv.shape, dtype=BF)
+    torch.cuda.synchronize()
+    for i in range(20):
+        for x, gr, st in zip(graphed, graphs, streams):
+            with torch.cuda.stream(st):
+                x.qkv.copy_(rows[i])
+                gr.replay()
+    torch.cuda.synchronize()
+    for i in range(20):
+        for x in eager:
+            x.qkv.copy_(rows[i])
+            x.step()
+    assert all(same_budgets(x, y) for x, y in zip(graphed, eager))
+
+
+def test_evict_with_scratch_on_two_streams_and_in_graphs():
+    """Contexts whose keys shared memory does not hold: eager on two streams at
+    once, then two graphs at once, against the oracle."""
+    cases = [([45001, 41000], 2000, 100), ([43777, 50000], 41000, 3)]
+    states = [evict_inputs(lens, 1, 64, BF, seed=i) for i, (lens, _, _) in enumerate(cases)]
+    want = [ref.kv_evict(*s, b, rec, 4) for s, (_, b, rec) in zip(states, cases)]
+    work = [[t.clone() for t in s] for s in states]
+    streams = [torch.cuda.Stream() for _ in cases]
+    lens = [torch.empty_like(s[5]) for s in states]
+
+    def evict(i):
+        for t, s in zip(work[i][:4], states[i][:4]):
+            t.copy_(s)
+        ops.kv_evict(*work[i], cases[i][1], cases[i][2], sink=4, new_lens=lens[i])
+
+    def check():
+        torch.cuda.synchronize()
+        for i, w in enumerate(want):
+            assert all(torch.equal(a, b) for a, b in zip((*work[i][:4], lens[i]), w))
+            for t in work[i][:4]:
+                t.zero_()
+            lens[i].zero_()
+        torch.cuda.synchronize()
+
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                for _ in range(4):
+                    evict(i)
+        check()
+    graphs = []
+    for i in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            evict(i)
+        graphs.append(gr)
+    for _ in range(3):
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                for _ in range(4):
+                    gr.replay()
+        check()

@@ -133,3 +133,19 @@ def test_evict_refuses_missing_pointers(lib, name):
 
 def test_calls_without_work_do_nothing(lib):
     assert append(lib, T=0) == 0 and scored(lib, R=0) == 0 and scored(lib, Q=0) == 0 and evict(lib, R=0) == 0
+
+
+@pytest.mark.parametrize("R,Q,Hq,Hkv,D,max_len,kernels", [
+    (3, 1, 8, 2, 128, 48, 1), (16, 1, 8, 2, 128, 224, 1), (2, 1, 8, 2, 128, 912, 1),      # short decode loops
+    (4, 1, 8, 2, 128, 5008, 1), (200, 1, 8, 8, 64, 176, 1),
+    (300, 1, 8, 2, 128, 224, 2), (1, 1, 32, 8, 128, 12000, 2), (40, 1, 32, 8, 128, 1664, 2),
+    (64, 1, 32, 8, 128, 20000, 2), (2, 16, 8, 2, 128, 6000, 2)])
+def test_form_of_a_scored_call(lib, R, Q, Hq, Hkv, D, max_len, kernels):
+    """Which calls take one kernel (and no scratch) on 148 SMs: what the GPU
+    tests of scratch, streams and graphs rely on."""
+    assert (lib.sched_attn_scored_ws_floats(R, Q, Hq, Hkv, D, max_len, 148) > 0) == (kernels == 2)
+
+
+@pytest.mark.parametrize("max_len,budget,scratch", [(40960, 100, False), (40961, 100, True), (224, 200, False), (50000, 50000, False)])
+def test_evictions_that_need_scratch(lib, max_len, budget, scratch):
+    assert (lib.sched_kv_evict_ws_ints(2, 1, max_len, budget, 148) > 0) == scratch
