@@ -283,6 +283,9 @@ __global__ void __launch_bounds__(kNormThreads, PIPE ? kNormResident : 6) qk_nor
 // 3.4 us with one head, 3.6 with two, 4.5 with four in the pipeline; 1024
 // tokens 8.6, 6.6, 7.3; 4097 tokens 31, 25.6, 22.7; 8000 tokens 64, 47, 37
 // (5.4 TB/s; copying as many bytes takes 18 us for 4097 tokens, 33 for 8000).
+// The pipeline takes about 5.7 us to start and drain and 3.95 us for each stride of
+// the resident lane groups over 987 tokens (6.3 TB/s): 17.3 us for three
+// strides, 21.7 for four, 25.6 for five; 4097 tokens are 4.15.
 template <typename T, int D>
 int run_qk_norm(const QkNormArgs &a, cudaStream_t st) {
   const long long lanes = (long long)a.T * (a.Hq + 2 * a.Hkv) * (D / 16);
@@ -318,6 +321,7 @@ constexpr int kTile = 16;      // tokens per warp step: divides the page size
 // 1664 tokens, 8 heads of 128, 4 query rows each 78 us with three, 90 with two,
 // 121 with four (spills); 16 rows 115 with two, 126 with three. 4 heads of 64,
 // 64 x 4000 tokens: 4 rows 61 us with four, 69 with three; 16 rows 85 and 89.
+// (168 registers with three CTAs: 8 rows of 128 spill 16 to 24 bytes.)
 constexpr int resident(int D, int block) { return D == 64 ? 4 : block == 16 ? 2 : 3; }
 constexpr int kMinRun = 2;     // tiles per warp at least: bounds the partial results
 
@@ -341,10 +345,12 @@ inline ScoredPlan scored_plan(int R, int Q, int Hq, int Hkv, int D, int max_len,
   const long long most = (tasks * (p.lp / kTile) + kMinRun * kWarps - 1) / (kMinRun * kWarps);
   const long long fill = (long long)num_sms * resident(D, p.block);
   p.grid = (int)(most < fill ? most : fill);
-  // the join's CTAs all resident at once where that is possible, with each thread having a logit to read
+  // The join's CTAs all resident at once where that is possible, with each thread having a logit to read. Sized by
+  // max_len: of very uneven batches the long requests' weights are few CTAs' work (one request of 32768 tokens among
+  // 63 of 100, 8 heads of 128, 4 rows: 86 us, against 38 alone).
   p.join = p.rows >= 16 ? 64 : p.rows >= 8 ? 128 : p.rows >= 4 ? 256 : p.rows >= 2 ? 512 : 1024;
   while (heads * ((max_len + p.join - 1) / p.join) > 4ll * num_sms && p.join < max_len) p.join += p.join < 1024 ? p.join : 1024;
-  // and at most 16 partial results per warp
+  // and at most 16 partial results per warp, by the average of the tasks (a long request's rows have more)
   p.o_rows = 1;
   while (p.o_rows < 32 && heads * ((p.rows + p.o_rows - 1) / p.o_rows) > (p.o_rows < 8 ? 1 : 4) * num_sms &&
          p.grid * kWarps / tasks * p.o_rows * 2 <= 8 * 16)
@@ -678,8 +684,10 @@ struct RowSoftmax {
 
 // One warp: a run of the tile list. Memory bound: 64 requests of 1536 to 1664
 // tokens (8 heads of 128, 4 query rows each) take 71 us, 92 % of the copy
-// rate, 8 of up to 32768 (8 rows) 150 us, 93 %. With 16 rows the products,
-// exponentials and logits of a tile take longer than its loads (115 us).
+// rate, 8 of up to 32768 (8 rows) 150 us, 93 %. With 16 rows the registers
+// leave 8 warps an SM, whose one tile ahead does not cover the loads' latency:
+// the same 64 requests 95 us at 25 % of the issue slots, 14 % of the tensor
+// pipe and 3.5 warps waiting for loads per issue.
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kWarps * 32, resident(D, ROWS))
     scored_split_kernel(const ScoredArgs a, const ScoredPlan pl) {
@@ -1171,9 +1179,11 @@ __host__ __device__ __forceinline__ size_t evict_words(int n) { return (size_t)(
 // prefix sum over the flags ranks both.
 //
 // Measured: 64 requests of 2112 slots to 2048, 8 heads of 128: 19 us, of which
-// reading scores and positions would take 3: the rest is the issue and the
-// barriers of the selection. 16 of 8192 to 2048: 52 us, 14 of selection and
-// then 206 MB of moves at the copy rate.
+// reading scores and positions would take 3. Its 512 CTAs are one wave and in
+// the same phase at once; warps wait for loads (3.0 per issue) and at barriers
+// (2.3), with 49 % of the issue slots used. 16 of 8192 to 2048: 52 us, 14 of
+// selection and then 206 MB of moves in 38, 83 % of the copy rate: 128 CTAs of
+// 1024 threads, one to an SM, leave 20 SMs without one.
 template <int D, bool IN_WS>
 __global__ void __launch_bounds__(1024) evict_kernel(const KvEvictArgs a, uint32_t *ws, int vec, int page_shift) {
   extern __shared__ __align__(16) uint32_t dyn[];  // evict_words(max_len) unless they are in the workspace (IN_WS)
@@ -1547,8 +1557,8 @@ inline OneKernel one_kernel(int R, int Hkv, int D, const ScoredPlan &pl, int num
   const long long heads = (long long)R * Hkv;
   // Eight CTAs of eight warps: one to an SM with heads of 128 (by its
   // registers), two with 64, and of the SMs about three quarters, since a
-  // cluster lies within a GPC (14 clusters of one-to-an-SM CTAs fit, 16 do
-  // not). One request of 700 tokens, 8 heads of 128: 6.4 us against 9.3 with
+  // cluster lies within a GPC (of 148 SMs 14 clusters of one-to-an-SM CTAs fit,
+  // which the 8 below admits; 16 do not). One request of 700 tokens, 8 heads of 128: 6.4 us against 9.3 with
   // two kernels, of 8000: 19.2 against 20.7; 16 such heads of 1000 tokens,
   // which do not fit: 12.5 against 11.6.
   if (tiles_of(8, 8) <= kCTiles) {
@@ -1565,7 +1575,7 @@ inline OneKernel one_kernel(int R, int Hkv, int D, const ScoredPlan &pl, int num
   for (int c = 4; c >= 1; c /= 2) {
     const int tiles = tiles_of(c, 4);
     if (tiles > kCTiles) break;
-    const int per_sm = D == 64 && pl.block == 16 && tiles > 4 ? 3 : one_resident(D, 4);  // (3: shared memory)
+    const int per_sm = D == 64 && pl.block == 16 && tiles > 4 ? 3 : one_resident(D, 4);  // (3: 57 KB of shared memory each)
     const long long capacity = (long long)per_sm * num_sms;
     if (heads * c <= capacity && (tiles <= 4 || heads * c * 2 > capacity)) return form(c, 4);
   }
