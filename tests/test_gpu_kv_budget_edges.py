@@ -9,7 +9,7 @@ import torch
 
 from sched_pass_b200 import _ext, ops
 from sched_pass_b200.models import reference as ref
-from test_gpu_kv_budget import (BF, DEV, FP, Budget, evict_inputs, expect_bad_index, gen, i32, paged, randn, rope_table,
+from test_gpu_kv_budget import (BF, DEV, FP, Budget, check_scored, evict_inputs, expect_bad_index, gen, i32, paged, randn, rope_table,
                                 run_scored, scored_inputs)
 
 pytestmark = pytest.mark.gpu
@@ -314,3 +314,52 @@ def test_evict_with_scratch_on_two_streams_and_in_graphs():
                 for _ in range(4):
                     gr.replay()
         check()
+
+
+# ------------------------------------------------------------------ outputs in place, long caches
+@pytest.mark.parametrize("T", [3, 900, 4200])
+def test_append_into_the_rows_that_it_reads(T):
+    """q_out as a view of the projection's own rows: the query heads turn in place."""
+    Hq, Hkv, D = 12, 4, 128
+    g = gen(T)
+    rows = randn(g, T, (Hq + 2 * Hkv) * D, dtype=BF)
+    wq, wk = (1 + 0.2 * randn(g, D)).to(BF), (1 + 0.2 * randn(g, D)).to(BF)
+    pos = torch.randint(0, 64, (T,), generator=g, device=DEV).to(torch.int32)
+    slot = torch.randperm(T + 7, generator=g, device=DEV)[:T].to(torch.int32)
+    P, cs = -(-(T + 7) // 16), rope_table(64, D)
+    caches = [torch.zeros(P, Hkv, 16, D, dtype=BF, device=DEV) for _ in range(4)]
+    q = torch.empty(T, Hq, D, dtype=BF, device=DEV)
+    ops.qk_norm_rope_kv_append(rows, wq, wk, 1e-5, pos, slot, cs, q, *caches[:2], Hq, Hkv)
+    own = rows.clone()
+    ops.qk_norm_rope_kv_append(own, wq, wk, 1e-5, pos, slot, cs, own[:, :Hq * D].view(T, Hq, D), *caches[2:], Hq, Hkv)
+    assert torch.equal(own[:, :Hq * D].view(T, Hq, D), q) and torch.equal(own[:, Hq * D:], rows[:, Hq * D:])
+    assert torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+
+
+@pytest.mark.parametrize("lens,Q,Hq,Hkv,D", [([700, 33], 1, 8, 2, 128), ([1600] * 40, 1, 32, 8, 64), ([300, 2000] * 9, 6, 16, 2, 128)])
+def test_scored_output_over_its_queries(lens, Q, Hq, Hkv, D):
+    q, kc, vc, bt, kl, scores0 = scored_inputs(lens, Q, Hq, Hkv, D, BF)
+    want, s1, s2 = torch.empty_like(q), scores0.clone(), scores0.clone()
+    ops.attention_decode_scored(q, want, kc, vc, bt, kl, D**-0.5, s1)
+    ops.attention_decode_scored(q, q, kc, vc, bt, kl, D**-0.5, s2)
+    assert torch.equal(q, want) and torch.equal(s1, s2)
+
+
+def test_scored_two_kernels_with_offsets_past_32_bits():
+    P, Hkv, D, n = 270000, 8, 128, 3000
+    kc = torch.empty(P, Hkv, 16, D, dtype=BF, device=DEV)
+    vc, scores = torch.empty_like(kc), torch.zeros(P, Hkv, 16, device=DEV)
+    last = P - 1 - torch.randperm(188, generator=gen(1), device=DEV)
+    g = gen(2)
+    kc[last], vc[last] = randn(g, 188, Hkv, 16, D, dtype=BF), randn(g, 188, Hkv, 16, D, dtype=BF)
+    small = kc[last].clone(), vc[last].clone()
+    table = torch.zeros(60, 188, dtype=torch.int32, device=DEV)
+    table[7] = last.to(torch.int32)
+    lens = i32([0] * 7 + [n] + [0] * 52)
+    q = randn(g, 60, 1, 16, D, dtype=BF)
+    out, n0 = torch.empty_like(q), _ext.launches()
+    ops.attention_decode_scored(q, out, kc, vc, table, lens, D**-0.5, scores)
+    assert _ext.launches() - n0 == 2
+    check_scored(q[7:8], *small, torch.arange(188, dtype=torch.int32, device=DEV)[None], i32([n]),
+                 torch.zeros(188, Hkv, 16, device=DEV), out[7:8], None, scores[last], D**-0.5)
+    assert out[:7].abs().max() == 0 and out[8:].abs().max() == 0
